@@ -18,6 +18,7 @@ VORTEX_LIB_PATH = os.path.join(_HERE, "libakili_vortex.so")
 ABI_VERSION = 1
 DTYPE_F32 = 0
 DTYPE_F16 = 1
+DTYPE_BF16 = 2  # the serving entries (include/akili_serving.h)
 
 OK = 0
 E_NULL_ARG = -1
@@ -163,6 +164,80 @@ class Kb2GemmSiluMulArg(C.Structure):  # benchmarks/kb2_gemm_silu_mul/common.h
                        ("c_addr", _u64)]
 
 
+# ---- serving structs (include/akili_serving.h); stride arrays as one field per axis ----
+_i64, _d = C.c_int64, C.c_double
+ROPE_INTERLEAVED, ROPE_INVERSE = 1, 2
+ROPE_SCALINGS = {None: 0, "linear": 1, "base": 2, "bands": 3, "ramp": 4}
+STATUS_BAD_INDEX = 0x2001
+
+
+def _axes(name, *axes):
+    return [(f"{name}_{a}", _i64) for a in axes]
+
+
+class RopeArg(C.Structure):  # akili_rope_arg_t
+    _fields_ = [("dtype", _u32), ("flags", _u32), ("tokens", _u32), ("q_heads", _u32), ("k_heads", _u32),
+                ("head_dim", _u32), ("rot_dim", _u32), ("max_positions", _u32), ("q_addr", _u64), ("k_addr", _u64),
+                ("q_out_addr", _u64), ("k_out_addr", _u64), ("positions_addr", _u64), ("table_addr", _u64),
+                *_axes("q_stride", "token", "head"), *_axes("k_stride", "token", "head"),
+                *_axes("q_out_stride", "token", "head"), *_axes("k_out_stride", "token", "head"), ("v_addr", _u64),
+                ("slots_addr", _u64), ("k_pages_addr", _u64), ("v_pages_addr", _u64), ("num_pages", _u32),
+                ("page_size", _u32), *_axes("v_stride", "token", "head"),
+                *_axes("k_page_stride", "page", "token", "head"), *_axes("v_page_stride", "page", "token", "head")]
+
+
+class RopeTableArg(C.Structure):  # akili_rope_table_arg_t
+    _fields_ = [("max_positions", _u32), ("rot_dim", _u32), ("scaling", _u32), ("reserved", _u32), ("base", _d),
+                ("factor", _d), ("original_positions", _d), ("low", _d), ("high", _d), ("amplitude", _d),
+                ("table_addr", _u64)]
+
+
+class PromptAttentionArg(C.Structure):  # akili_prompt_attention_arg_t
+    _fields_ = [("dtype", _u32), ("q_heads", _u32), ("kv_heads", _u32), ("head_dim", _u32), ("batch", _u32),
+                ("total_q", _u32), ("total_k", _u32), ("causal", _u32), ("softmax_scale", _f), ("reserved", _u32),
+                ("q_addr", _u64), ("k_addr", _u64), ("v_addr", _u64), ("o_addr", _u64), ("lse_addr", _u64),
+                ("cu_q_addr", _u64), ("cu_k_addr", _u64), *_axes("q_stride", "token", "head"),
+                *_axes("k_stride", "token", "head"), *_axes("v_stride", "token", "head"),
+                *_axes("o_stride", "token", "head")]
+
+
+class TreeAttentionArg(C.Structure):  # akili_tree_attention_arg_t
+    _fields_ = [("dtype", _u32), ("q_heads", _u32), ("kv_heads", _u32), ("head_dim", _u32), ("batch", _u32),
+                ("total_q", _u32), ("num_pages", _u32), ("page_size", _u32), ("max_pages", _u32),
+                ("mask_words", _u32), ("softmax_scale", _f), ("reserved", _u32), ("q_addr", _u64),
+                ("k_pages_addr", _u64), ("v_pages_addr", _u64), ("o_addr", _u64), ("lse_addr", _u64),
+                ("page_table_addr", _u64), ("context_lens_addr", _u64), ("cu_q_addr", _u64), ("mask_addr", _u64),
+                ("workspace", _u64), ("workspace_bytes", _u64), *_axes("q_stride", "token", "head"),
+                *_axes("o_stride", "token", "head"), *_axes("k_page_stride", "page", "token", "head"),
+                *_axes("v_page_stride", "page", "token", "head"), ("page_table_stride", _i64), ("mask_stride", _i64)]
+
+
+class TreeMaskArg(C.Structure):  # akili_tree_mask_arg_t
+    _fields_ = [("batch", _u32), ("total_q", _u32), ("mask_words", _u32), ("reserved", _u32), ("parents_addr", _u64),
+                ("cu_q_addr", _u64), ("mask_addr", _u64)]
+
+
+class CacheAcceptArg(C.Structure):  # akili_cache_accept_arg_t
+    _fields_ = [("elem_bytes", _u32), ("layers", _u32), ("batch", _u32), ("kv_heads", _u32), ("head_dim", _u32),
+                ("num_pages", _u32), ("page_size", _u32), ("max_pages", _u32), ("max_accepted", _u32),
+                ("reserved", _u32), ("k_pages_addr", _u64), ("v_pages_addr", _u64), ("page_table_addr", _u64),
+                ("context_lens_addr", _u64), ("accepted_addr", _u64), ("n_accepted_addr", _u64),
+                ("new_lens_addr", _u64), *_axes("k_page_stride", "layer", "page", "token", "head"),
+                *_axes("v_page_stride", "layer", "page", "token", "head"), ("page_table_stride", _i64),
+                ("accepted_stride", _i64)]
+
+
+# name -> (struct, sizeof in C)
+SERVING_OPS = {
+    "rope": (RopeArg, 248),
+    "rope_append": (RopeArg, 248),
+    "rope_table": (RopeTableArg, 72),
+    "prompt_attention": (PromptAttentionArg, 160),
+    "tree_attention": (TreeAttentionArg, 232),
+    "tree_mask": (TreeMaskArg, 40),
+    "cache_accept": (CacheAcceptArg, 176),
+}
+
 # name -> (struct, buffer fields in harness upload order + outputs, sizeof in the reference)
 OPS = {
     "kbt_sgemm": (KbtSgemmArg, 64),
@@ -208,6 +283,12 @@ def load(path: str = LIB_PATH) -> C.CDLL:
         fx = getattr(L, f"akili_{name}_ex")
         fx.argtypes = [C.POINTER(st), C.POINTER(AkiliEx), C.c_void_p]
         fx.restype = C.c_int
+    for name, (st, _) in SERVING_OPS.items():
+        f = getattr(L, f"akili_{name}")
+        f.argtypes = [C.POINTER(st), C.c_void_p]
+        f.restype = C.c_int
+    L.akili_tree_attention_workspace.argtypes = [C.POINTER(TreeAttentionArg), C.POINTER(C.c_uint64)]
+    L.akili_tree_attention_workspace.restype = C.c_int
     L.akili_attention.argtypes = [C.POINTER(AttentionArg), C.c_void_p]
     L.akili_attention.restype = C.c_int
     L.akili_attention_ex.argtypes = [C.POINTER(AttentionArg), C.POINTER(AkiliEx), C.c_void_p]

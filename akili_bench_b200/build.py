@@ -40,7 +40,7 @@ VXMATH_LIB = os.path.join(HERE, "libakili_vxmath.so")
 
 def _sources():
     return [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith((".cu", ".cuh"))] + \
-        [os.path.join(ROOT, "include", "akili.h")]
+        [os.path.join(ROOT, "include", h) for h in ("akili.h", "akili_serving.h")]
 
 
 def _stale(out: str, deps: list[str]) -> bool:

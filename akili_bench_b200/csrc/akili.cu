@@ -26,6 +26,7 @@
 #include <utility>
 
 #include "../../include/akili.h"
+#include "../../include/akili_serving.h"
 #include "attention_unfused.cuh"
 #include "aux.cuh"
 #include "flash.cuh"
@@ -1954,6 +1955,7 @@ int akili_device_status(uint32_t* status, int clear) {
     unsigned int z = 0;
     if (cudaMemcpyToSymbol(g_status, &z, sizeof(z)) != cudaSuccess) return AKILI_E_LAUNCH;
   }
+  if (v == AKILI_STATUS_BAD_INDEX) return AKILI_E_SHAPE;
   return v ? AKILI_E_DEVICE_TIMEOUT : AKILI_OK;
 }
 
@@ -1991,3 +1993,5 @@ int akili_sm_clock_read(uint64_t* cycles, uint64_t* ns, int clear) {
 uint32_t akili_abi_version(void) { return AKILI_ABI_VERSION; }
 
 }  // extern "C"
+
+#include "serving_host.cuh"

@@ -1,0 +1,361 @@
+// serving_host.cuh — the entries of include/akili_serving.h: argument checks
+// and launches.  Included by akili.cu (shares its device, scratch and
+// tensor-map helpers).
+#pragma once
+#include "../../include/akili_serving.h"
+#include "cache.cuh"
+#include "rope.cuh"
+#include "serving_attention.cuh"
+
+namespace {
+
+int serving_elem_bytes(uint32_t dtype) {
+  return dtype == AKILI_DTYPE_F32 ? 4 : dtype == AKILI_DTYPE_F16 || dtype == AKILI_DTYPE_BF16 ? 2 : 0;
+}
+
+int check_aligned(std::initializer_list<uint64_t> ps, uint64_t bytes) {
+  for (uint64_t p : ps)
+    if (p == 0) return AKILI_E_NULL_ARG;
+  for (uint64_t p : ps)
+    if (p % bytes) return AKILI_E_ALIGN;
+  return AKILI_OK;
+}
+
+template <size_t n>
+bool all_multiples(const int64_t (&st)[n], int64_t of) {
+  for (int64_t s : st)
+    if (s % of) return false;
+  return true;
+}
+
+// ------------------------------------------------------------------- rope --
+template <typename T, int VEC, bool kAppend>
+int launch_rope(const DevInfo& di, const RopeArgs& r, cudaStream_t st) {
+  const int units = r.rot_dim / 2 / VEC + (r.head_dim - r.rot_dim + 2 * VEC - 1) / (2 * VEC);
+  const int hl = kRopeThreads / std::min(units, kRopeThreads);
+  const int heads = r.q_heads + r.k_heads * (kAppend ? 2 : 1);
+  // few tokens: the heads of one are shared among as many blocks as they fill
+  const int most = (heads + hl - 1) / hl;
+  const int want = (4 * di.sms + r.tokens - 1) / r.tokens;
+  const dim3 grid(r.tokens, std::min({most, want, 65535}));
+  rope_kernel<T, VEC, kAppend><<<grid, kRopeThreads, 0, st>>>(r);
+  return launch_status();
+}
+
+template <typename T, bool kAppend>
+int launch_rope_vec(const DevInfo& di, const RopeArgs& r, bool vec, cudaStream_t st) {
+  return vec ? launch_rope<T, 16 / sizeof(T), kAppend>(di, r, st) : launch_rope<T, 1, kAppend>(di, r, st);
+}
+
+int run_rope(const akili_rope_arg_t* a, bool append, cudaStream_t st) {
+  if (!a) return AKILI_E_NULL_ARG;
+  const int es = serving_elem_bytes(a->dtype);
+  if (!es) return AKILI_E_DTYPE;
+  if (a->flags & ~(AKILI_ROPE_INTERLEAVED | AKILI_ROPE_INVERSE)) return AKILI_E_UNSUPPORTED;
+  if (a->rot_dim == 0 || a->rot_dim % 2 || a->rot_dim > a->head_dim || a->max_positions == 0) return AKILI_E_SHAPE;
+  if (a->tokens > INT32_MAX || a->head_dim > 65536 || a->q_heads > 65536 || a->k_heads > 65536 ||
+      a->max_positions > INT32_MAX)
+    return AKILI_E_SHAPE;
+  if (append && (a->page_size == 0 || a->page_size > INT32_MAX || a->num_pages > INT32_MAX)) return AKILI_E_SHAPE;
+  if (a->tokens == 0 || (a->q_heads == 0 && a->k_heads == 0)) return AKILI_OK;
+  int rc;
+  if ((rc = check_aligned({a->positions_addr, a->table_addr}, 4))) return rc;
+  if (a->q_heads && (rc = check_aligned({a->q_addr, a->q_out_addr}, es))) return rc;
+  if (a->k_heads && (rc = check_aligned({a->k_addr}, es))) return rc;
+  if (a->k_heads && !append && (rc = check_aligned({a->k_out_addr}, es))) return rc;
+  if (a->k_heads && append && (rc = check_aligned({a->v_addr, a->k_pages_addr, a->v_pages_addr}, es))) return rc;
+  if (append && (rc = check_aligned({a->slots_addr}, 8))) return rc;
+  DevInfo di;
+  if ((rc = device_info(&di))) return rc;
+  RopeArgs r{};
+  r.q = P(a->q_addr); r.k = P(a->k_addr); r.v = P(a->v_addr);
+  r.q_out = W(a->q_out_addr);
+  r.k_out = W(append ? a->k_pages_addr : a->k_out_addr);
+  r.v_out = W(a->v_pages_addr);
+  r.positions = static_cast<const int*>(P(a->positions_addr));
+  r.table = F(a->table_addr);
+  r.slots = static_cast<const long long*>(P(a->slots_addr));
+  r.tokens = a->tokens; r.q_heads = a->q_heads; r.k_heads = a->k_heads;
+  r.head_dim = a->head_dim; r.rot_dim = a->rot_dim; r.max_positions = a->max_positions;
+  r.num_pages = a->num_pages; r.page_size = a->page_size;
+  r.interleaved = (a->flags & AKILI_ROPE_INTERLEAVED) != 0;
+  r.sin_sign = (a->flags & AKILI_ROPE_INVERSE) ? -1.0f : 1.0f;
+  for (int i = 0; i < 2; ++i) {
+    r.q_st[i] = a->q_stride[i]; r.k_st[i] = a->k_stride[i]; r.qo_st[i] = a->q_out_stride[i];
+    r.v_st[i] = a->v_stride[i];
+    r.ko_st[i + 1] = a->k_out_stride[i];
+  }
+  if (append)
+    for (int i = 0; i < 3; ++i) { r.ko_st[i] = a->k_page_stride[i]; r.vo_st[i] = a->v_page_stride[i]; }
+  // 16-byte accesses where every vector of every head starts on 16 bytes
+  const int64_t n = 16 / es;
+  bool vec = (a->rot_dim / 2) % n == 0 && (a->head_dim - a->rot_dim) % n == 0 && a->head_dim / (2 * n) <= kRopeThreads;
+  if (a->q_heads)
+    vec = vec && (a->q_addr | a->q_out_addr) % 16 == 0 && all_multiples(a->q_stride, n) &&
+          all_multiples(a->q_out_stride, n);
+  if (a->k_heads) {
+    vec = vec && a->k_addr % 16 == 0 && all_multiples(a->k_stride, n);
+    if (append)
+      vec = vec && (a->v_addr | a->k_pages_addr | a->v_pages_addr) % 16 == 0 && all_multiples(a->v_stride, n) &&
+            all_multiples(a->k_page_stride, n) && all_multiples(a->v_page_stride, n);
+    else
+      vec = vec && a->k_out_addr % 16 == 0 && all_multiples(a->k_out_stride, n);
+  }
+  if (a->dtype == AKILI_DTYPE_F32)
+    return append ? launch_rope_vec<float, true>(di, r, vec, st) : launch_rope_vec<float, false>(di, r, vec, st);
+  if (a->dtype == AKILI_DTYPE_F16)
+    return append ? launch_rope_vec<__half, true>(di, r, vec, st) : launch_rope_vec<__half, false>(di, r, vec, st);
+  return append ? launch_rope_vec<__nv_bfloat16, true>(di, r, vec, st)
+                : launch_rope_vec<__nv_bfloat16, false>(di, r, vec, st);
+}
+
+int run_rope_table(const akili_rope_table_arg_t* a, cudaStream_t st) {
+  if (!a) return AKILI_E_NULL_ARG;
+  if (a->scaling > AKILI_ROPE_SCALE_RAMP || a->reserved) return AKILI_E_UNSUPPORTED;
+  if (a->max_positions == 0 || a->max_positions > INT32_MAX || a->rot_dim == 0 || a->rot_dim % 2 ||
+      a->rot_dim > kRopeMaxRot)
+    return AKILI_E_SHAPE;
+  const auto positive = [](double x) { return x > 0.0 && std::isfinite(x); };
+  if (!positive(a->base) || !(a->amplitude >= 0.0) || !std::isfinite(a->amplitude)) return AKILI_E_UNSUPPORTED;
+  if (a->scaling != AKILI_ROPE_SCALE_NONE && !positive(a->factor)) return AKILI_E_UNSUPPORTED;
+  if (a->scaling == AKILI_ROPE_SCALE_BASE && a->rot_dim == 2) return AKILI_E_UNSUPPORTED;
+  if (a->scaling >= AKILI_ROPE_SCALE_BANDS &&
+      (!positive(a->original_positions) || !positive(a->low) || !positive(a->high) || a->high <= a->low))
+    return AKILI_E_UNSUPPORTED;
+  if (a->scaling == AKILI_ROPE_SCALE_RAMP && a->base <= 1.0) return AKILI_E_UNSUPPORTED;
+  int rc;
+  if ((rc = check_aligned({a->table_addr}, 4))) return rc;
+  DevInfo di;
+  if ((rc = device_info(&di))) return rc;
+  RopeTableArgs t{};
+  const int half = a->rot_dim / 2;
+  const double r = a->rot_dim, two_pi = 6.283185307179586;
+  double base = a->base;
+  if (a->scaling == AKILI_ROPE_SCALE_BASE) base *= std::pow(a->factor, r / (r - 2.0));
+  // RAMP: the pair that turns n times within original_positions is
+  // i(n) = r ln(original / (2 pi n)) / (2 ln base)
+  double lo = 0.0, hi = 0.0;
+  if (a->scaling == AKILI_ROPE_SCALE_RAMP) {
+    const auto pair_of = [&](double turns) {
+      return r * std::log(a->original_positions / (two_pi * turns)) / (2.0 * std::log(base));
+    };
+    lo = std::max(std::floor(pair_of(a->high)), 0.0);
+    hi = std::min(std::ceil(pair_of(a->low)), r - 1.0);
+    if (hi <= lo) hi = lo + 0.001;
+  }
+  for (int i = 0; i < half; ++i) {
+    double f = std::pow(base, -2.0 * i / r);
+    if (a->scaling == AKILI_ROPE_SCALE_LINEAR) f /= a->factor;
+    if (a->scaling == AKILI_ROPE_SCALE_BANDS) {
+      const double turns = a->original_positions * f / two_pi;  // original / wavelength
+      const double keep = std::min(std::max((turns - a->low) / (a->high - a->low), 0.0), 1.0);
+      f = keep * f + (1.0 - keep) * f / a->factor;
+    }
+    if (a->scaling == AKILI_ROPE_SCALE_RAMP) {
+      const double slow = std::min(std::max((i - lo) / (hi - lo), 0.0), 1.0);
+      f = slow * f / a->factor + (1.0 - slow) * f;
+    }
+    t.freq[i] = f;
+  }
+  t.amplitude = a->amplitude != 0.0 ? a->amplitude
+                : a->scaling == AKILI_ROPE_SCALE_RAMP && a->factor > 1.0 ? 0.1 * std::log(a->factor) + 1.0
+                                                                         : 1.0;
+  t.table = static_cast<float*>(W(a->table_addr));
+  t.max_positions = a->max_positions;
+  t.rot_dim = a->rot_dim;
+  rope_table_kernel<<<grid_for(di, static_cast<size_t>(a->max_positions) * half, 256, 8), 256, 0, st>>>(t);
+  return launch_status();
+}
+
+// ------------------------------------------------------------------ cache --
+int run_tree_mask(const akili_tree_mask_arg_t* a, cudaStream_t st) {
+  if (!a) return AKILI_E_NULL_ARG;
+  if (a->reserved) return AKILI_E_UNSUPPORTED;
+  if (a->total_q > INT32_MAX - 128 || a->batch > INT32_MAX || a->mask_words == 0 || a->mask_words > 65536)
+    return AKILI_E_SHAPE;
+  if (a->total_q == 0) return AKILI_OK;
+  if (a->batch == 0) return AKILI_E_SHAPE;
+  int rc;
+  if ((rc = check_aligned({a->parents_addr, a->cu_q_addr, a->mask_addr}, 4))) return rc;
+  DevInfo di;
+  if ((rc = device_info(&di))) return rc;
+  tree_mask_kernel<<<(a->total_q + 127) / 128, 128, 0, st>>>(
+      static_cast<const int*>(P(a->parents_addr)), static_cast<const int*>(P(a->cu_q_addr)),
+      static_cast<unsigned int*>(W(a->mask_addr)), a->batch, a->total_q, a->mask_words);
+  return launch_status();
+}
+
+template <typename U>
+int launch_accept(const DevInfo& di, AcceptArgs g, const akili_cache_accept_arg_t* a, cudaStream_t st) {
+  g.vecs = static_cast<int>(a->head_dim * a->elem_bytes / sizeof(U));
+  const int64_t cols = 2ll * a->kv_heads * g.vecs;
+  const int share = static_cast<int>(std::min<int64_t>((cols + kAcceptThreads - 1) / kAcceptThreads, 1024));
+  cache_accept_kernel<U><<<dim3(share, a->batch, a->layers), kAcceptThreads, 0, st>>>(g);
+  (void)di;
+  return launch_status();
+}
+
+int run_cache_accept(const akili_cache_accept_arg_t* a, cudaStream_t st) {
+  if (!a) return AKILI_E_NULL_ARG;
+  if (a->reserved) return AKILI_E_UNSUPPORTED;
+  if (a->elem_bytes != 1 && a->elem_bytes != 2 && a->elem_bytes != 4) return AKILI_E_DTYPE;
+  if (a->page_size == 0 || a->kv_heads == 0 || a->head_dim == 0 || a->layers == 0 || a->max_pages == 0)
+    return AKILI_E_SHAPE;
+  if (a->layers > 65535 || a->batch > 65535 || a->kv_heads > 65536 || a->head_dim > 8192 ||
+      a->page_size > INT32_MAX || a->num_pages > INT32_MAX || a->max_pages > INT32_MAX || a->max_accepted > INT32_MAX)
+    return AKILI_E_SHAPE;
+  if (a->batch == 0) return AKILI_OK;
+  int rc;
+  if ((rc = check_aligned({a->k_pages_addr, a->v_pages_addr}, a->elem_bytes))) return rc;
+  if ((rc = check_aligned({a->page_table_addr, a->context_lens_addr, a->n_accepted_addr}, 4))) return rc;
+  if (a->max_accepted && (rc = check_aligned({a->accepted_addr}, 4))) return rc;
+  if (a->new_lens_addr % 4) return AKILI_E_ALIGN;
+  if (a->new_lens_addr == a->context_lens_addr) return AKILI_E_UNSUPPORTED;
+  DevInfo di;
+  if ((rc = device_info(&di))) return rc;
+  AcceptArgs g{};
+  g.k = static_cast<char*>(W(a->k_pages_addr));
+  g.v = static_cast<char*>(W(a->v_pages_addr));
+  g.page_table = static_cast<const int*>(P(a->page_table_addr));
+  g.context_lens = static_cast<const int*>(P(a->context_lens_addr));
+  g.accepted = static_cast<const int*>(P(a->accepted_addr));
+  g.n_accepted = static_cast<const int*>(P(a->n_accepted_addr));
+  g.new_lens = static_cast<int*>(W(a->new_lens_addr));
+  g.kv_heads = a->kv_heads; g.num_pages = a->num_pages; g.page_size = a->page_size;
+  g.max_pages = a->max_pages; g.max_accepted = a->max_accepted;
+  uint64_t bits = a->k_pages_addr | a->v_pages_addr | (a->head_dim * a->elem_bytes);
+  for (int i = 0; i < 4; ++i) {
+    g.k_st[i] = a->k_page_stride[i] * a->elem_bytes;
+    g.v_st[i] = a->v_page_stride[i] * a->elem_bytes;
+    bits |= static_cast<uint64_t>(g.k_st[i] | g.v_st[i]);
+  }
+  g.table_stride = a->page_table_stride;
+  g.acc_stride = a->accepted_stride;
+  // 16-byte moves where every head row starts on 16 bytes, else element by element
+  if (bits % 16 == 0) return launch_accept<uint4>(di, g, a, st);
+  if (a->elem_bytes == 4) return launch_accept<uint32_t>(di, g, a, st);
+  if (a->elem_bytes == 2) return launch_accept<uint16_t>(di, g, a, st);
+  return launch_accept<uint8_t>(di, g, a, st);
+}
+
+// -------------------------------------------------------------- attention --
+int check_heads(uint32_t dtype, uint32_t hq, uint32_t hk, uint32_t d, float scale) {
+  if (dtype != AKILI_DTYPE_F16 && dtype != AKILI_DTYPE_BF16) return AKILI_E_DTYPE;
+  if (hq == 0 || hk == 0 || hq % hk || d == 0 || d % 8) return AKILI_E_SHAPE;
+  if (d > 128 || hq > 65535) return AKILI_E_UNSUPPORTED;
+  if (!(scale >= 0.0f) || !std::isfinite(scale)) return AKILI_E_UNSUPPORTED;
+  return AKILI_OK;
+}
+
+float scale_log2_of(float scale, uint32_t d) {
+  return (scale != 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(d))) * 1.4426950408889634f;
+}
+
+template <bool kPaged>
+int launch_attention_rows(const ServingArgs& g, uint32_t dtype, cudaStream_t st) {
+  const int64_t rows = static_cast<int64_t>(g.total_q) * g.q_heads;
+  const unsigned blocks = static_cast<unsigned>((rows + 3) / 4);
+  if (dtype == AKILI_DTYPE_F16) attention_rows_kernel<__half, kPaged><<<blocks, 128, 0, st>>>(g);
+  else attention_rows_kernel<__nv_bfloat16, kPaged><<<blocks, 128, 0, st>>>(g);
+  return launch_status();
+}
+
+int run_prompt_attention(const akili_prompt_attention_arg_t* a, cudaStream_t st) {
+  if (!a) return AKILI_E_NULL_ARG;
+  int rc;
+  if ((rc = check_heads(a->dtype, a->q_heads, a->kv_heads, a->head_dim, a->softmax_scale))) return rc;
+  if (a->causal > 1 || a->reserved) return AKILI_E_UNSUPPORTED;
+  if (a->total_q > (1u << 30) || a->total_k > (1u << 30) || a->batch > (1u << 20)) return AKILI_E_SHAPE;
+  if (a->batch == 0 && a->total_q) return AKILI_E_SHAPE;
+  if (a->total_q == 0) return AKILI_OK;
+  if ((rc = check_ptrs({a->q_addr, a->o_addr}))) return rc;
+  if (a->total_k && (rc = check_ptrs({a->k_addr, a->v_addr}))) return rc;
+  if ((rc = check_aligned({a->cu_q_addr, a->cu_k_addr}, 4))) return rc;
+  if (a->lse_addr % 4) return AKILI_E_ALIGN;
+  if (!all_multiples(a->q_stride, 8) || !all_multiples(a->k_stride, 8) || !all_multiples(a->v_stride, 8) ||
+      !all_multiples(a->o_stride, 8))
+    return AKILI_E_ALIGN;
+  DevInfo di;
+  if ((rc = device_info(&di))) return rc;
+  ServingArgs g{};
+  g.q = P(a->q_addr); g.k = P(a->k_addr); g.v = P(a->v_addr); g.o = W(a->o_addr);
+  g.lse = static_cast<float*>(W(a->lse_addr));
+  g.cu_q = static_cast<const int*>(P(a->cu_q_addr));
+  g.cu_k = static_cast<const int*>(P(a->cu_k_addr));
+  g.q_heads = a->q_heads; g.kv_heads = a->kv_heads; g.head_dim = a->head_dim; g.batch = a->batch;
+  g.total_q = a->total_q; g.total_k = a->total_k; g.causal = a->causal;
+  g.scale_log2 = scale_log2_of(a->softmax_scale, a->head_dim);
+  for (int i = 0; i < 2; ++i) {
+    g.q_st[i] = a->q_stride[i]; g.o_st[i] = a->o_stride[i];
+    g.k_st[i + 1] = a->k_stride[i]; g.v_st[i + 1] = a->v_stride[i];
+  }
+  return launch_attention_rows<false>(g, a->dtype, st);
+}
+
+int check_tree(const akili_tree_attention_arg_t* a) {
+  if (!a) return AKILI_E_NULL_ARG;
+  int rc;
+  if ((rc = check_heads(a->dtype, a->q_heads, a->kv_heads, a->head_dim, a->softmax_scale))) return rc;
+  if (a->reserved) return AKILI_E_UNSUPPORTED;
+  if (a->page_size == 0 || a->page_size % 8 || a->page_size > (1u << 20) || a->max_pages == 0 || a->num_pages == 0)
+    return AKILI_E_SHAPE;
+  if (a->total_q > (1u << 30) || a->batch > (1u << 20) || a->num_pages > INT32_MAX || a->max_pages > INT32_MAX ||
+      static_cast<uint64_t>(a->max_pages) * a->page_size > (1u << 30) || a->mask_words > 65536)
+    return AKILI_E_SHAPE;
+  if (a->batch == 0 && a->total_q) return AKILI_E_SHAPE;
+  return AKILI_OK;
+}
+
+int run_tree_attention(const akili_tree_attention_arg_t* a, cudaStream_t st) {
+  int rc;
+  if ((rc = check_tree(a))) return rc;
+  if (a->total_q == 0) return AKILI_OK;
+  if ((rc = check_ptrs({a->q_addr, a->k_pages_addr, a->v_pages_addr, a->o_addr}))) return rc;
+  if ((rc = check_aligned({a->page_table_addr, a->context_lens_addr, a->cu_q_addr}, 4))) return rc;
+  if (a->lse_addr % 4 || a->mask_addr % 4) return AKILI_E_ALIGN;
+  if (a->mask_addr && a->mask_words == 0) return AKILI_E_SHAPE;
+  if (!all_multiples(a->q_stride, 8) || !all_multiples(a->o_stride, 8) || !all_multiples(a->k_page_stride, 8) ||
+      !all_multiples(a->v_page_stride, 8))
+    return AKILI_E_ALIGN;
+  DevInfo di;
+  if ((rc = device_info(&di))) return rc;
+  ServingArgs g{};
+  g.q = P(a->q_addr); g.k = P(a->k_pages_addr); g.v = P(a->v_pages_addr); g.o = W(a->o_addr);
+  g.lse = static_cast<float*>(W(a->lse_addr));
+  g.cu_q = static_cast<const int*>(P(a->cu_q_addr));
+  g.ctx = static_cast<const int*>(P(a->context_lens_addr));
+  g.page_table = static_cast<const int*>(P(a->page_table_addr));
+  g.mask = static_cast<const unsigned int*>(P(a->mask_addr));
+  g.q_heads = a->q_heads; g.kv_heads = a->kv_heads; g.head_dim = a->head_dim; g.batch = a->batch;
+  g.total_q = a->total_q;
+  g.num_pages = a->num_pages; g.page_size = a->page_size; g.max_pages = a->max_pages; g.mask_words = a->mask_words;
+  g.scale_log2 = scale_log2_of(a->softmax_scale, a->head_dim);
+  for (int i = 0; i < 2; ++i) { g.q_st[i] = a->q_stride[i]; g.o_st[i] = a->o_stride[i]; }
+  for (int i = 0; i < 3; ++i) { g.k_st[i] = a->k_page_stride[i]; g.v_st[i] = a->v_page_stride[i]; }
+  g.table_stride = a->page_table_stride;
+  g.mask_stride = a->mask_stride;
+  return launch_attention_rows<true>(g, a->dtype, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+int akili_rope(const akili_rope_arg_t* a, akili_stream_t s) { return run_rope(a, false, S(s)); }
+int akili_rope_append(const akili_rope_arg_t* a, akili_stream_t s) { return run_rope(a, true, S(s)); }
+int akili_rope_table(const akili_rope_table_arg_t* a, akili_stream_t s) { return run_rope_table(a, S(s)); }
+int akili_prompt_attention(const akili_prompt_attention_arg_t* a, akili_stream_t s) {
+  return run_prompt_attention(a, S(s));
+}
+int akili_tree_attention(const akili_tree_attention_arg_t* a, akili_stream_t s) { return run_tree_attention(a, S(s)); }
+int akili_tree_attention_workspace(const akili_tree_attention_arg_t* a, uint64_t* bytes) {
+  if (!bytes) return AKILI_E_NULL_ARG;
+  const int rc = check_tree(a);
+  if (rc) return rc;
+  *bytes = 0;
+  return AKILI_OK;
+}
+int akili_tree_mask(const akili_tree_mask_arg_t* a, akili_stream_t s) { return run_tree_mask(a, S(s)); }
+int akili_cache_accept(const akili_cache_accept_arg_t* a, akili_stream_t s) { return run_cache_accept(a, S(s)); }
+
+}  // extern "C"

@@ -16,6 +16,8 @@ import threading
 import torch
 
 from . import abi
+from .serving import (cache_accept, prompt_attention, rope, rope_append, rope_table,  # noqa: F401
+                      tree_attention, tree_attention_workspace, tree_mask)
 
 
 def _stream(stream) -> int:
