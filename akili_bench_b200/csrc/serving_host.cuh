@@ -239,6 +239,9 @@ int run_cache_accept(const akili_cache_accept_arg_t* a, cudaStream_t st) {
 }
 
 // -------------------------------------------------------------- attention --
+// Keys and values of the key heads that are scheduled together: half of L2.
+constexpr uint64_t kPromptChunkBytes = 64ull << 20;
+
 int check_heads(uint32_t dtype, uint32_t hq, uint32_t hk, uint32_t d, float scale) {
   if (dtype != AKILI_DTYPE_F16 && dtype != AKILI_DTYPE_BF16) return AKILI_E_DTYPE;
   if (hq == 0 || hk == 0 || hq % hk || d == 0 || d % 8) return AKILI_E_SHAPE;
@@ -251,13 +254,74 @@ float scale_log2_of(float scale, uint32_t d) {
   return (scale != 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(d))) * 1.4426950408889634f;
 }
 
-template <bool kPaged>
-int launch_attention_rows(const ServingArgs& g, uint32_t dtype, cudaStream_t st) {
-  const int64_t rows = static_cast<int64_t>(g.total_q) * g.q_heads;
-  const unsigned blocks = static_cast<unsigned>((rows + 3) / 4);
-  if (dtype == AKILI_DTYPE_F16) attention_rows_kernel<__half, kPaged><<<blocks, 128, 0, st>>>(g);
-  else attention_rows_kernel<__nv_bfloat16, kPaged><<<blocks, 128, 0, st>>>(g);
-  return launch_status();
+// [d3][d2][d1][d0] tensor of 16-bit values with these strides (elements), box
+// [1][1][box1][64], 128-byte swizzle.  The stride of an axis of one entry is never used.
+bool map_heads(CUtensorMap* m, const void* ptr, uint32_t dtype, int rank, const uint64_t (&dim)[4],
+               const int64_t (&stride)[3], int box_axis, uint32_t box) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return false;
+  cuuint64_t dims[4], strides[3];
+  cuuint32_t boxes[4] = {64, 1, 1, 1}, es[4] = {1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) dims[i] = dim[i];
+  for (int i = 0; i + 1 < rank; ++i) strides[i] = dim[i + 1] == 1 ? (dim[0] * 2 + 15) / 16 * 16 : stride[i] * 2;
+  boxes[box_axis] = box;
+  return enc(m, dtype == AKILI_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+             const_cast<void*>(ptr), dims, strides, boxes, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DP, typename T, bool kPaged, bool kPair>
+int launch_serving(const CUtensorMap& tk, const CUtensorMap& tv, const ServingArgs& g, int blocks, cudaStream_t st) {
+  auto kern = serving_attention_kernel<DP, T, kPaged, kPair>;
+  constexpr int smem = SvSmem<DP, kPair>::kBytes;
+  static std::mutex mu;
+  static std::map<int, bool> attr_done;
+  {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::lock_guard<std::mutex> lock(mu);
+    if (!attr_done[dev]) {
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+        cudaGetLastError();
+        return AKILI_E_LAUNCH;
+      }
+      attr_done[dev] = true;
+    }
+  }
+  kern<<<blocks, kSvThreads, smem, st>>>(tk, tv, g);
+  int rc = launch_status();
+  if constexpr (kPaged) {
+    if (rc) return rc;
+    // a programmatic dependent: its blocks are dispatched, and find their cut
+    // item, while the parts are still being computed
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(blocks, kSvJoinSplit);
+    cfg.blockDim = dim3(kSvJoinThreads);
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, attention_join_kernel<DP, T, kPair>, g) != cudaSuccess) {
+      cudaGetLastError();
+      return AKILI_E_LAUNCH;
+    }
+    rc = launch_status();
+  }
+  return rc;
+}
+
+template <bool kPaged, bool kPair>
+int launch_serving_typed(uint32_t dtype, const CUtensorMap& tk, const CUtensorMap& tv, const ServingArgs& g, int blocks,
+                         cudaStream_t st) {
+  const bool bf = dtype == AKILI_DTYPE_BF16;
+  if (g.head_dim <= 64)
+    return bf ? launch_serving<64, __nv_bfloat16, kPaged, kPair>(tk, tv, g, blocks, st)
+              : launch_serving<64, __half, kPaged, kPair>(tk, tv, g, blocks, st);
+  return bf ? launch_serving<128, __nv_bfloat16, kPaged, kPair>(tk, tv, g, blocks, st)
+            : launch_serving<128, __half, kPaged, kPair>(tk, tv, g, blocks, st);
 }
 
 int run_prompt_attention(const akili_prompt_attention_arg_t* a, cudaStream_t st) {
@@ -277,19 +341,32 @@ int run_prompt_attention(const akili_prompt_attention_arg_t* a, cudaStream_t st)
     return AKILI_E_ALIGN;
   DevInfo di;
   if ((rc = device_info(&di))) return rc;
+  const uint64_t group = a->q_heads / a->kv_heads;
+  const uint64_t blocks = ((a->total_q * group + 2 * kSvRows - 1) / (2 * kSvRows) + a->batch) * a->kv_heads;
+  if (a->total_q * group > (1u << 30) || blocks > INT32_MAX) return AKILI_E_SHAPE;
   ServingArgs g{};
-  g.q = P(a->q_addr); g.k = P(a->k_addr); g.v = P(a->v_addr); g.o = W(a->o_addr);
+  g.q = P(a->q_addr); g.o = W(a->o_addr);
   g.lse = static_cast<float*>(W(a->lse_addr));
   g.cu_q = static_cast<const int*>(P(a->cu_q_addr));
   g.cu_k = static_cast<const int*>(P(a->cu_k_addr));
-  g.q_heads = a->q_heads; g.kv_heads = a->kv_heads; g.head_dim = a->head_dim; g.batch = a->batch;
+  g.q_heads = a->q_heads; g.kv_heads = a->kv_heads; g.group = static_cast<int>(group);
+  g.head_dim = a->head_dim; g.batch = a->batch;
   g.total_q = a->total_q; g.total_k = a->total_k; g.causal = a->causal;
   g.scale_log2 = scale_log2_of(a->softmax_scale, a->head_dim);
-  for (int i = 0; i < 2; ++i) {
-    g.q_st[i] = a->q_stride[i]; g.o_st[i] = a->o_stride[i];
-    g.k_st[i + 1] = a->k_stride[i]; g.v_st[i + 1] = a->v_stride[i];
-  }
-  return launch_attention_rows<false>(g, a->dtype, st);
+  for (int i = 0; i < 2; ++i) { g.q_st[i] = a->q_stride[i]; g.o_st[i] = a->o_stride[i]; }
+  const uint64_t per_head = static_cast<uint64_t>(a->total_k) * a->head_dim * 4;  // bytes of K and V
+  g.chunk_heads = static_cast<int>(
+      std::min<uint64_t>(std::max<uint64_t>(kPromptChunkBytes / std::max<uint64_t>(per_head, 1), 1), a->kv_heads));
+  // without any key the maps are never used; they are made over q then
+  const bool keys = a->total_k > 0;
+  const uint64_t dim[4] = {a->head_dim, keys ? a->kv_heads : 1, keys ? a->total_k : 1, 1};
+  CUtensorMap tk, tv;
+  if (!map_heads(&tk, P(keys ? a->k_addr : a->q_addr), a->dtype, 3, dim, {a->k_stride[1], a->k_stride[0], 0}, 2,
+                 kSvKeys) ||
+      !map_heads(&tv, P(keys ? a->v_addr : a->q_addr), a->dtype, 3, dim, {a->v_stride[1], a->v_stride[0], 0}, 2,
+                 kSvKeys))
+    return AKILI_E_LAUNCH;
+  return launch_serving_typed<false, true>(a->dtype, tk, tv, g, static_cast<int>(blocks), st);
 }
 
 int check_tree(const akili_tree_attention_arg_t* a) {
@@ -303,7 +380,20 @@ int check_tree(const akili_tree_attention_arg_t* a) {
       static_cast<uint64_t>(a->max_pages) * a->page_size > (1u << 30) || a->mask_words > 65536)
     return AKILI_E_SHAPE;
   if (a->batch == 0 && a->total_q) return AKILI_E_SHAPE;
+  if (static_cast<uint64_t>(a->total_q) * (a->q_heads / a->kv_heads) > (1u << 30)) return AKILI_E_SHAPE;
   return AKILI_OK;
+}
+
+// Two row tiles per CTA when the rows of a (sequence, key head) fill more than
+// one on average, else both streams on one.
+bool tree_pair_form(const akili_tree_attention_arg_t* a) {
+  return static_cast<uint64_t>(a->total_q) * (a->q_heads / a->kv_heads) > static_cast<uint64_t>(kSvRows) * a->batch;
+}
+
+// Two parts (O, m, l) for each share of the line of key blocks.
+size_t tree_workspace_bytes(const DevInfo& di, const akili_tree_attention_arg_t* a) {
+  const size_t rows = (tree_pair_form(a) ? 2 : 1) * kSvRows;
+  return 2ull * di.sms * rows * ((a->head_dim <= 64 ? 64 : 128) + 2) * sizeof(float);
 }
 
 int run_tree_attention(const akili_tree_attention_arg_t* a, cudaStream_t st) {
@@ -319,22 +409,38 @@ int run_tree_attention(const akili_tree_attention_arg_t* a, cudaStream_t st) {
     return AKILI_E_ALIGN;
   DevInfo di;
   if ((rc = device_info(&di))) return rc;
+  const bool pair = tree_pair_form(a);
+  Mode md;
+  md.workspace = W(a->workspace);
+  md.workspace_bytes = a->workspace ? a->workspace_bytes : 0;
+  char* parts = nullptr;
+  if ((rc = acquire_scratch(md, tree_workspace_bytes(di, a), st, &parts))) return rc;
   ServingArgs g{};
-  g.q = P(a->q_addr); g.k = P(a->k_pages_addr); g.v = P(a->v_pages_addr); g.o = W(a->o_addr);
+  g.q = P(a->q_addr); g.o = W(a->o_addr);
   g.lse = static_cast<float*>(W(a->lse_addr));
   g.cu_q = static_cast<const int*>(P(a->cu_q_addr));
   g.ctx = static_cast<const int*>(P(a->context_lens_addr));
   g.page_table = static_cast<const int*>(P(a->page_table_addr));
   g.mask = static_cast<const unsigned int*>(P(a->mask_addr));
-  g.q_heads = a->q_heads; g.kv_heads = a->kv_heads; g.head_dim = a->head_dim; g.batch = a->batch;
-  g.total_q = a->total_q;
+  g.parts = reinterpret_cast<float*>(parts);
+  g.q_heads = a->q_heads; g.kv_heads = a->kv_heads; g.group = static_cast<int>(a->q_heads / a->kv_heads);
+  g.head_dim = a->head_dim; g.batch = a->batch; g.total_q = a->total_q;
   g.num_pages = a->num_pages; g.page_size = a->page_size; g.max_pages = a->max_pages; g.mask_words = a->mask_words;
+  g.box_rows = 8;
+  while (g.box_rows < kSvKeys && a->page_size % (2 * g.box_rows) == 0) g.box_rows *= 2;
   g.scale_log2 = scale_log2_of(a->softmax_scale, a->head_dim);
   for (int i = 0; i < 2; ++i) { g.q_st[i] = a->q_stride[i]; g.o_st[i] = a->o_stride[i]; }
-  for (int i = 0; i < 3; ++i) { g.k_st[i] = a->k_page_stride[i]; g.v_st[i] = a->v_page_stride[i]; }
   g.table_stride = a->page_table_stride;
   g.mask_stride = a->mask_stride;
-  return launch_attention_rows<true>(g, a->dtype, st);
+  const uint64_t dim[4] = {a->head_dim, a->page_size, a->kv_heads, a->num_pages};
+  CUtensorMap tk, tv;
+  if (!map_heads(&tk, P(a->k_pages_addr), a->dtype, 4, dim,
+                 {a->k_page_stride[1], a->k_page_stride[2], a->k_page_stride[0]}, 1, g.box_rows) ||
+      !map_heads(&tv, P(a->v_pages_addr), a->dtype, 4, dim,
+                 {a->v_page_stride[1], a->v_page_stride[2], a->v_page_stride[0]}, 1, g.box_rows))
+    return AKILI_E_LAUNCH;
+  return pair ? launch_serving_typed<true, true>(a->dtype, tk, tv, g, di.sms, st)
+              : launch_serving_typed<true, false>(a->dtype, tk, tv, g, di.sms, st);
 }
 
 }  // namespace
@@ -352,7 +458,9 @@ int akili_tree_attention_workspace(const akili_tree_attention_arg_t* a, uint64_t
   if (!bytes) return AKILI_E_NULL_ARG;
   const int rc = check_tree(a);
   if (rc) return rc;
-  *bytes = 0;
+  DevInfo di;
+  if (const int no = device_info(&di)) return no;
+  *bytes = tree_workspace_bytes(di, a);
   return AKILI_OK;
 }
 int akili_tree_mask(const akili_tree_mask_arg_t* a, akili_stream_t s) { return run_tree_mask(a, S(s)); }
