@@ -13,14 +13,18 @@
 * ``libakili_vxmath.so`` csrc/vxmath_b200.cpp — the llama2 matmul offload
                          API (benchmarks/llama2/vxmath.h) on top of
                          libakili.so, for the unchanged llama2/llama.cpp.
+* ``_serving.so``        csrc/serving_torch.cpp — the torch front end of the
+                         serving operators (a CPython module over libakili.so).
 
 All land next to this file so they travel with the working tree.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -36,6 +40,7 @@ NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-shared"
 LIB = os.path.join(HERE, "libakili.so")
 VORTEX_LIB = os.path.join(HERE, "libakili_vortex.so")
 VXMATH_LIB = os.path.join(HERE, "libakili_vxmath.so")
+SERVING_MODULE = os.path.join(HERE, "_serving.so")
 
 
 def _sources():
@@ -75,7 +80,18 @@ def build(force: bool = False, verbose: bool = False) -> list[str]:
             if verbose:
                 print(" ".join(cmd))
             _run(cmd)
-    return [LIB, VORTEX_LIB, VXMATH_LIB]
+    src = os.path.join(CSRC, "serving_torch.cpp")
+    if force or _stale(SERVING_MODULE, [src, os.path.join(ROOT, "include", "akili_serving.h")]):
+        torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+        cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-I", os.path.join(ROOT, "include"), "-I",
+               os.path.join(torch_dir, "include"), "-I", os.path.join(torch_dir, "include/torch/csrc/api/include"), "-I",
+               sysconfig.get_paths()["include"], "-I", cuda_inc, src, "-o", SERVING_MODULE, "-L", HERE, "-lakili", "-L",
+               os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+               "-Wl,-rpath,$ORIGIN"]
+        if verbose:
+            print(" ".join(cmd))
+        _run(cmd)
+    return [LIB, VORTEX_LIB, VXMATH_LIB, SERVING_MODULE]
 
 
 if __name__ == "__main__":
