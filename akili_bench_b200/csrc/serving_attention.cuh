@@ -142,7 +142,8 @@ __device__ __forceinline__ void sv_streams(const ServingArgs& a, SvPiece& p, int
 }
 
 // A CTA's share of the line of key blocks; every role walks it by itself.
-template <bool kPair>
+// kTileRows: rows of an item (16 to 256).
+template <int kTileRows>
 struct SvWalk {
   long long pos, begin, end, off;  // off: position within sequence b
   int b;
@@ -154,7 +155,7 @@ struct SvWalk {
     bool clamped;
     s = sv_sequence<true>(a, b, &clamped);
     rows = s.n * a.group;
-    tiles = (rows + (kPair ? 2 : 1) * kSvRows - 1) / ((kPair ? 2 : 1) * kSvRows);
+    tiles = (rows + kTileRows - 1) / kTileRows;
     blocks = (s.m + kSvKeys - 1) / kSvKeys;
     size = static_cast<long long>(a.kv_heads) * tiles * blocks;
   }
@@ -171,11 +172,11 @@ struct SvWalk {
     p.s = s;
     p.b = b;
     p.hk = static_cast<int>(item / tiles);
-    p.row0 = static_cast<int>(item - static_cast<long long>(p.hk) * tiles) * ((kPair ? 2 : 1) * kSvRows);
+    p.row0 = static_cast<int>(item - static_cast<long long>(p.hk) * tiles) * kTileRows;
     p.rows = rows;
     p.kb = kb;
     p.part = take == blocks ? -1 : 2 * cta + (pos == begin ? 0 : 1);
-    sv_streams<true, kPair>(a, p, kb + take);
+    sv_streams<true, kTileRows == 2 * kSvRows>(a, p, kb + take);
     pos += take;
     off += take;
     return true;
@@ -198,10 +199,10 @@ __device__ __forceinline__ long long warp_scan(long long v) {  // inclusive
 }
 
 // Blocks of sequence b on the line (0 past the batch).
-template <bool kPair>
+template <int kTileRows>
 __device__ __forceinline__ long long sv_line_blocks(const ServingArgs& a, int b, bool record) {
   if (b >= a.batch) return 0;
-  SvWalk<kPair> w;
+  SvWalk<kTileRows> w;
   w.b = b;
   w.load(a);
   if (record) {
@@ -213,12 +214,12 @@ __device__ __forceinline__ long long sv_line_blocks(const ServingArgs& a, int b,
 }
 
 // The share of CTA `cta` of `ctas` (one warp): false if it is empty.
-template <bool kPair>
-__device__ __forceinline__ bool sv_share(const ServingArgs& a, int cta, int ctas, SvWalk<kPair>& w,
+template <int kTileRows>
+__device__ __forceinline__ bool sv_share(const ServingArgs& a, int cta, int ctas, SvWalk<kTileRows>& w,
                                          long long* quota_out, long long* total_out) {
   const int lane = threadIdx.x & 31;
   long long total = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 32) total += sv_line_blocks<kPair>(a, b0 + lane, cta == 0);
+  for (int b0 = 0; b0 < a.batch; b0 += 32) total += sv_line_blocks<kTileRows>(a, b0 + lane, cta == 0);
   total = warp_sum(total);
   const long long quota = (total + ctas - 1) / ctas;
   *quota_out = quota;
@@ -228,7 +229,7 @@ __device__ __forceinline__ bool sv_share(const ServingArgs& a, int cta, int ctas
   if (w.begin >= total) return false;
   long long before = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
-    const long long mine = sv_line_blocks<kPair>(a, b0 + lane, false);
+    const long long mine = sv_line_blocks<kTileRows>(a, b0 + lane, false);
     const long long upto = before + warp_scan(mine);
     const unsigned hit = __ballot_sync(0xffffffffu, upto > w.begin);
     if (hit) {
@@ -334,12 +335,16 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* m, uint64_t* bar, int x, int y, int z,
-                                            int w) {
+// Executed by the whole (converged) warp with warp-uniform operands; one
+// elected lane issues.
+__device__ __forceinline__ void tma_load_4d_warp(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int y, int z,
+                                                 int w) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, "
-      "%6}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(m), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, "
+      "%6}], [%2];\n\t}" ::"r"(dst),
+      "l"(m), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
       : "memory");
 }
 
@@ -358,6 +363,7 @@ __global__ void __maxnreg__(96)
     serving_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                              const __grid_constant__ ServingArgs a) {
   using L = SvSmem<DP, kPair>;
+  constexpr int kTileRows = (kPair ? 2 : 1) * kSvRows;
   constexpr int kStages = L::kStages;
   constexpr int kChunks = DP / 64;              // 64-column swizzle chunks
   constexpr int kParts = DP >= 128 ? 4 : 2;     // parts in which P is announced
@@ -383,9 +389,9 @@ __global__ void __maxnreg__(96)
   if (warp == 0) {
     bool work;
     if constexpr (kPaged) {
-      SvWalk<kPair> w;
+      SvWalk<kTileRows> w;
       long long quota, total;
-      work = sv_share<kPair>(a, cta, gridDim.x, w, &quota, &total);
+      work = sv_share<kTileRows>(a, cta, gridDim.x, w, &quota, &total);
       if (lane == 0 && work) {
         ctl->b = w.b;
         ctl->begin = w.begin;
@@ -433,7 +439,7 @@ __global__ void __maxnreg__(96)
   const bool work = ctl->work != 0;
 
   // The pieces of this CTA: one tile (prompts) or a share of the line (cache).
-  SvWalk<kPair> walk;
+  SvWalk<kTileRows> walk;
   int pieces = 0;
   if constexpr (kPaged) {
     if (work) {
@@ -474,19 +480,14 @@ __global__ void __maxnreg__(96)
         const uint32_t ph = (count / kStages) & 1;
         const int key0 = (pc.kb + j) * kSvKeys;
         uint32_t bytes = L::kKV;
-        int page = 0, row = 0, chunk = 0;
-        bool mine = lane == 0;
+        int page = 0, boxes = 0;
+        const bool mine = lane == 0;
         if constexpr (kPaged) {
-          // lane -> (box of box_rows keys, 64-column chunk): at most 16 x 2
-          const int per = kSvKeys / a.box_rows;
-          const int boxes = (min(kSvKeys, pc.s.m - key0) + a.box_rows - 1) / a.box_rows;
-          const int box = static_cast<int>(lane) % per;
-          chunk = static_cast<int>(lane) / per;
+          // lane b looks up the page of box b (box_rows keys)
+          boxes = (min(kSvKeys, pc.s.m - key0) + a.box_rows - 1) / a.box_rows;
           bytes = static_cast<uint32_t>(boxes * a.box_rows * 128 * kChunks);
-          mine = box < boxes && chunk < kChunks;
-          row = box * a.box_rows;
-          if (mine) {
-            const int key = key0 + row;
+          if (static_cast<int>(lane) < boxes) {
+            const int key = key0 + static_cast<int>(lane) * a.box_rows;
             page = a.page_table[pc.b * a.table_stride + key / a.page_size];
             if (page < 0 || page >= a.num_pages) {  // outside the tensor: TMA fills zeros
               record_bad_index();
@@ -500,10 +501,16 @@ __global__ void __maxnreg__(96)
           if (lane == 0) mbar_expect_tx(&full[st], bytes);
           __syncwarp();
           if constexpr (kPaged) {
-            const int in_page = (key0 + row) % a.page_size;
-            if (mine)
-              tma_load_4d(ring + st * L::kKV + chunk * 16384 + row * 128, &tm, &full[st], chunk * 64, in_page, pc.hk,
-                          page);
+            const uint32_t dst = smem_u32(ring + st * L::kKV), bar = smem_u32(&full[st]);
+            int in_page = key0 % a.page_size;
+#pragma unroll 4
+            for (int box = 0; box < boxes; ++box) {
+              const int at = __shfl_sync(0xffffffffu, page, box);
+              for (int c = 0; c < kChunks; ++c)
+                tma_load_4d_warp(dst + c * 16384 + box * a.box_rows * 128, &tm, bar, c * 64, in_page, pc.hk, at);
+              in_page += a.box_rows;
+              if (in_page == a.page_size) in_page = 0;
+            }
           } else {
             if (mine)
               for (int c = 0; c < kChunks; ++c)
@@ -802,7 +809,6 @@ __global__ void __maxnreg__(96)
       // the row's columns; with the single form the row's four threads have a
       // quarter each, of the sum of both streams.
       float* slot = nullptr;  // [kRows][DP] O, [kRows] m, [kRows] l
-      constexpr int kTileRows = (kPair ? 2 : 1) * kSvRows;
       if (kPaged && pc.part >= 0) slot = a.parts + static_cast<size_t>(pc.part) * kTileRows * (DP + 2);
       const int prow = (kPair ? grp * kSvRows : 0) + r;
       T* out = static_cast<T*>(a.o) + qrow * a.o_st[0] + head * a.o_st[1];
@@ -924,15 +930,14 @@ __global__ void __maxnreg__(96)
 // Adds up the parts of the item that starts in share c = blockIdx.x and goes
 // on past its end, in order: a warp per row, four values of the head per lane.
 //   m = max m_p,  o = sum 2^(m_p - m) O_p / sum 2^(m_p - m) l_p
-template <int DP, typename T, bool kPair>
+template <int DP, typename T, int kTileRows>
 __global__ void __launch_bounds__(kSvJoinThreads) attention_join_kernel(const __grid_constant__ ServingArgs a) {
-  constexpr int kTileRows = (kPair ? 2 : 1) * kSvRows;
   __shared__ int from, parts, slot0, row0, rows, q0, hk;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
-    SvWalk<kPair> w;
+    SvWalk<kTileRows> w;
     long long quota, total;
-    const bool work = sv_share<kPair>(a, blockIdx.x, gridDim.x, w, &quota, &total);
+    const bool work = sv_share<kTileRows>(a, blockIdx.x, gridDim.x, w, &quota, &total);
     if (lane == 0) {
       parts = 0;
       SvPiece p;

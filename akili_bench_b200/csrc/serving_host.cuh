@@ -4,6 +4,7 @@
 #pragma once
 #include "../../include/akili_serving.h"
 #include "cache.cuh"
+#include "decode_attention.cuh"
 #include "rope.cuh"
 #include "serving_attention.cuh"
 
@@ -271,57 +272,82 @@ bool map_heads(CUtensorMap* m, const void* ptr, uint32_t dtype, int rank, const 
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DP, typename T, bool kPaged, bool kPair>
-int launch_serving(const CUtensorMap& tk, const CUtensorMap& tv, const ServingArgs& g, int blocks, cudaStream_t st) {
-  auto kern = serving_attention_kernel<DP, T, kPaged, kPair>;
-  constexpr int smem = SvSmem<DP, kPair>::kBytes;
-  static std::mutex mu;
-  static std::map<int, bool> attr_done;
-  {
+// The attribute that grants a kernel its shared memory, once per device; `done`
+// belongs to one kernel.
+struct SmemGrant {
+  std::mutex mu;
+  std::map<int, bool> done;
+  int operator()(const void* kern, int bytes) {
     int dev = 0;
     cudaGetDevice(&dev);
     std::lock_guard<std::mutex> lock(mu);
-    if (!attr_done[dev]) {
-      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
-        cudaGetLastError();
-        return AKILI_E_LAUNCH;
-      }
-      attr_done[dev] = true;
-    }
-  }
-  kern<<<blocks, kSvThreads, smem, st>>>(tk, tv, g);
-  int rc = launch_status();
-  if constexpr (kPaged) {
-    if (rc) return rc;
-    // a programmatic dependent: its blocks are dispatched, and find their cut
-    // item, while the parts are still being computed
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(blocks, kSvJoinSplit);
-    cfg.blockDim = dim3(kSvJoinThreads);
-    cfg.stream = st;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, attention_join_kernel<DP, T, kPair>, g) != cudaSuccess) {
+    if (done[dev]) return AKILI_OK;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
       cudaGetLastError();
       return AKILI_E_LAUNCH;
     }
-    rc = launch_status();
+    done[dev] = true;
+    return AKILI_OK;
   }
-  return rc;
+};
+
+template <int DP, typename T>
+int launch_prompt(const CUtensorMap& tk, const CUtensorMap& tv, const ServingArgs& g, int blocks, cudaStream_t st) {
+  auto kern = serving_attention_kernel<DP, T, false, true>;
+  constexpr int smem = SvSmem<DP, true>::kBytes;
+  static SmemGrant grant;
+  if (const int rc = grant(reinterpret_cast<const void*>(kern), smem)) return rc;
+  kern<<<blocks, kSvThreads, smem, st>>>(tk, tv, g);
+  return launch_status();
 }
 
-template <bool kPaged, bool kPair>
-int launch_serving_typed(uint32_t dtype, const CUtensorMap& tk, const CUtensorMap& tv, const ServingArgs& g, int blocks,
-                         cudaStream_t st) {
-  const bool bf = dtype == AKILI_DTYPE_BF16;
-  if (g.head_dim <= 64)
-    return bf ? launch_serving<64, __nv_bfloat16, kPaged, kPair>(tk, tv, g, blocks, st)
-              : launch_serving<64, __half, kPaged, kPair>(tk, tv, g, blocks, st);
-  return bf ? launch_serving<128, __nv_bfloat16, kPaged, kPair>(tk, tv, g, blocks, st)
-            : launch_serving<128, __half, kPaged, kPair>(tk, tv, g, blocks, st);
+// The attention over a cache with items of kTileRows rows, then the join of
+// its cut items.
+template <int DP, typename T, int kTileRows>
+int launch_cache(const CUtensorMap& tk, const CUtensorMap& tv, const ServingArgs& g, int blocks, cudaStream_t st) {
+  static SmemGrant grant;
+  int rc;
+  if constexpr (kTileRows >= kSvRows) {
+    constexpr bool kPair = kTileRows > kSvRows;
+    auto kern = serving_attention_kernel<DP, T, true, kPair>;
+    constexpr int smem = SvSmem<DP, kPair>::kBytes;
+    if ((rc = grant(reinterpret_cast<const void*>(kern), smem))) return rc;
+    kern<<<blocks, kSvThreads, smem, st>>>(tk, tv, g);
+  } else {
+    auto kern = decode_attention_kernel<DP, T, kTileRows>;
+    constexpr int smem = DcSmem<DP, kTileRows>::kBytes;
+    if ((rc = grant(reinterpret_cast<const void*>(kern), smem))) return rc;
+    kern<<<blocks, kDcThreads, smem, st>>>(tk, tv, g);
+  }
+  if ((rc = launch_status())) return rc;
+  // a programmatic dependent: its blocks are dispatched, and find their cut
+  // item, while the parts are still being computed
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(blocks, kSvJoinSplit);
+  cfg.blockDim = dim3(kSvJoinThreads);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, attention_join_kernel<DP, T, kTileRows>, g) != cudaSuccess) {
+    cudaGetLastError();
+    return AKILI_E_LAUNCH;
+  }
+  return launch_status();
+}
+
+template <int DP, typename T>
+int launch_cache_rows(int rows, const CUtensorMap& tk, const CUtensorMap& tv, const ServingArgs& g, int blocks,
+                      cudaStream_t st) {
+  switch (rows) {
+    case 16: return launch_cache<DP, T, 16>(tk, tv, g, blocks, st);
+    case 32: return launch_cache<DP, T, 32>(tk, tv, g, blocks, st);
+    case 64: return launch_cache<DP, T, 64>(tk, tv, g, blocks, st);
+    case 128: return launch_cache<DP, T, 128>(tk, tv, g, blocks, st);
+    default: return launch_cache<DP, T, 256>(tk, tv, g, blocks, st);
+  }
 }
 
 int run_prompt_attention(const akili_prompt_attention_arg_t* a, cudaStream_t st) {
@@ -366,7 +392,11 @@ int run_prompt_attention(const akili_prompt_attention_arg_t* a, cudaStream_t st)
       !map_heads(&tv, P(keys ? a->v_addr : a->q_addr), a->dtype, 3, dim, {a->v_stride[1], a->v_stride[0], 0}, 2,
                  kSvKeys))
     return AKILI_E_LAUNCH;
-  return launch_serving_typed<false, true>(a->dtype, tk, tv, g, static_cast<int>(blocks), st);
+  const int n = static_cast<int>(blocks);
+  if (a->dtype == AKILI_DTYPE_BF16)
+    return g.head_dim <= 64 ? launch_prompt<64, __nv_bfloat16>(tk, tv, g, n, st)
+                            : launch_prompt<128, __nv_bfloat16>(tk, tv, g, n, st);
+  return g.head_dim <= 64 ? launch_prompt<64, __half>(tk, tv, g, n, st) : launch_prompt<128, __half>(tk, tv, g, n, st);
 }
 
 int check_tree(const akili_tree_attention_arg_t* a) {
@@ -384,16 +414,19 @@ int check_tree(const akili_tree_attention_arg_t* a) {
   return AKILI_OK;
 }
 
-// Two row tiles per CTA when the rows of a (sequence, key head) fill more than
-// one on average, else both streams on one.
-bool tree_pair_form(const akili_tree_attention_arg_t* a) {
-  return static_cast<uint64_t>(a->total_q) * (a->q_heads / a->kv_heads) > static_cast<uint64_t>(kSvRows) * a->batch;
+// Rows of an item (tokens times grouped heads of one key head): the smallest
+// form that holds the mean of the sequences.  The host does not know the
+// single lengths; a longer sequence takes several items.
+int tree_tile_rows(const akili_tree_attention_arg_t* a) {
+  const uint64_t rows = static_cast<uint64_t>(a->total_q) * (a->q_heads / a->kv_heads);
+  int form = 16;
+  while (form < 2 * kSvRows && rows > static_cast<uint64_t>(form) * a->batch) form *= 2;
+  return form;
 }
 
 // Two parts (O, m, l) for each share of the line of key blocks.
 size_t tree_workspace_bytes(const DevInfo& di, const akili_tree_attention_arg_t* a) {
-  const size_t rows = (tree_pair_form(a) ? 2 : 1) * kSvRows;
-  return 2ull * di.sms * rows * ((a->head_dim <= 64 ? 64 : 128) + 2) * sizeof(float);
+  return 2ull * di.sms * tree_tile_rows(a) * ((a->head_dim <= 64 ? 64 : 128) + 2) * sizeof(float);
 }
 
 int run_tree_attention(const akili_tree_attention_arg_t* a, cudaStream_t st) {
@@ -409,7 +442,6 @@ int run_tree_attention(const akili_tree_attention_arg_t* a, cudaStream_t st) {
     return AKILI_E_ALIGN;
   DevInfo di;
   if ((rc = device_info(&di))) return rc;
-  const bool pair = tree_pair_form(a);
   Mode md;
   md.workspace = W(a->workspace);
   md.workspace_bytes = a->workspace ? a->workspace_bytes : 0;
@@ -439,8 +471,12 @@ int run_tree_attention(const akili_tree_attention_arg_t* a, cudaStream_t st) {
       !map_heads(&tv, P(a->v_pages_addr), a->dtype, 4, dim,
                  {a->v_page_stride[1], a->v_page_stride[2], a->v_page_stride[0]}, 1, g.box_rows))
     return AKILI_E_LAUNCH;
-  return pair ? launch_serving_typed<true, true>(a->dtype, tk, tv, g, di.sms, st)
-              : launch_serving_typed<true, false>(a->dtype, tk, tv, g, di.sms, st);
+  const int rows = tree_tile_rows(a);
+  if (a->dtype == AKILI_DTYPE_BF16)
+    return g.head_dim <= 64 ? launch_cache_rows<64, __nv_bfloat16>(rows, tk, tv, g, di.sms, st)
+                            : launch_cache_rows<128, __nv_bfloat16>(rows, tk, tv, g, di.sms, st);
+  return g.head_dim <= 64 ? launch_cache_rows<64, __half>(rows, tk, tv, g, di.sms, st)
+                          : launch_cache_rows<128, __half>(rows, tk, tv, g, di.sms, st);
 }
 
 }  // namespace

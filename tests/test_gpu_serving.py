@@ -389,6 +389,35 @@ def test_tree_attention(dtype, case):
         at += n
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hk,new", [(5, 1, 3), (16, 1, 1), (4, 2, 11), (8, 2, 13), (3, 1, 40), (8, 2, 50), (16, 2, 33)])
+def test_tree_attention_row_forms_and_rising_scores(dtype, d, hq, hk, new):
+    """Every row form (16 to 256 rows of an item), scores that rise along the context (the running maximum
+    moves in most blocks) or fall, contexts that are cut between CTAs and ones that are not."""
+    g = gen(hq * 100 + new)
+    ctx = [2500, 0, 260, 77]
+    for tree, rise in ((True, True), (False, True), (True, False)):
+        kp, vp, table, ks, vs = make_cache(g, [c + new for c in ctx], 16, hk, d, dtype)
+        for b, c in enumerate(ctx):  # scale entry j's key by its place
+            f = (torch.arange(c + new) + 1.0) / 40.0
+            f = (f if rise else f.flip(0))[:, None, None]
+            ks[b] = (ks[b].abs() * f).to(dtype)
+            for j in range(c + new):
+                kp[int(table[b, j // 16]), j % 16] = ks[b][j].cuda()
+        q = normal(g, (4 * new, hq, d), dtype).abs()
+        parents = [random_parents(g, new) for _ in ctx]
+        cu = prefix([new] * 4).cuda()
+        mask = ops.tree_mask(i32(sum(parents, [])).cuda(), cu, new) if tree else None
+        got, lse = ops.tree_attention(q.cuda(), kp, vp, table.cuda(), i32(ctx).cuda(), cu, mask, softmax_scale=0.02,
+                                      return_lse=True)
+        for b, c in enumerate(ctx):
+            seen = ref.tree_seen(c, parents[b]) if tree else ref.causal(new, c + new)
+            o, l, bound, l_bound = ref.attend(q[b * new:(b + 1) * new], ks[b], vs[b], seen, 0.02)
+            ref.assert_within(got[b * new:(b + 1) * new], o, bound, f"sequence {b}")
+            ref.assert_within(lse[b * new:(b + 1) * new], l, l_bound, f"lse of sequence {b}")
+
+
 def test_tree_mask_bits():
     g = gen(20)
     new = [1, 40, 0, 97, 32]
