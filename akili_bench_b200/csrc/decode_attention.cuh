@@ -189,7 +189,8 @@ __global__ void __launch_bounds__(kDcThreads, 1)
     walk.end = ctl->end;
     walk.off = ctl->off;
     walk.b = ctl->b;
-    walk.load(a);
+    bool clamped;
+    walk.load(a, &clamped);
   }
   SvPiece pc;
   auto next = [&]() { return work && walk.next(a, blockIdx.x, pc); };
@@ -352,9 +353,9 @@ __global__ void __launch_bounds__(kDcThreads, 1)
 #pragma unroll 4
       for (int x = lane; x < kUnits; x += 32) {
         const int n = x / (DP / 8), c = x % (DP / 8);
-        const int row = pc.row0 + n;
+        const int row = pc.tile * N + n;
         uint4 v = {0, 0, 0, 0};
-        if (row < pc.rows && c * 8 < a.head_dim) {
+        if (row < pc.s.n * a.group && c * 8 < a.head_dim) {
           const int tok = row / a.group;
           const int head = pc.hk * a.group + row - tok * a.group;
           v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (pc.s.q0 + tok) * a.q_st[0] +
@@ -384,9 +385,10 @@ __global__ void __launch_bounds__(kDcThreads, 1)
         m[n] = -3.4028235e38f;  // "nothing seen": any finite score passes it
         l[n] = 0.0f;
       }
-      const int tok0 = pc.row0 / a.group;
-      const int rem0 = pc.row0 - tok0 * a.group;
-      const int nrows = min(N, pc.rows - pc.row0);
+      const int row0 = pc.tile * N;
+      const int tok0 = row0 / a.group;
+      const int rem0 = row0 - tok0 * a.group;
+      const int nrows = min(N, pc.s.n * a.group - row0);
       // keys that every row sees
       const int common = tree ? pc.s.sure : min(pc.s.m, pc.s.sure + tok0 + 1);
       for (int j = 0; j < pc.loads; ++j, ++g) {

@@ -3,43 +3,51 @@
 //
 //   o_i = sum_j softmax_j(scale q_i.k_j) v_j   over the keys j that i sees
 //
-// Rows.  The G = q_heads / kv_heads query heads of a key head share its keys,
-// so the rows of a (sequence, key head) are its tokens times G: row r is
-// token r / G, head r % G of the group.  Short sequences and single tokens
-// fill the 128-row tiles of the tensor core that way, keys are loaded once
-// for the group, and a causal tile spans few tokens, so that its diagonal
-// wastes little.
+// This file holds the forms with the query rows on the M side of the tensor
+// core; decode_attention.cuh the one for few rows.
 //
-// One CTA per SM, 576 threads, two streams of scores, each with its own S/P
+// Rows.  The G = q_heads / kv_heads query heads of a key head share its keys,
+// so the rows of a 128-row tile are tokens times P heads, P = G (or its
+// largest divisor up to 128): row r is token r / P, head r % P of the group.
+// Short sequences fill the tensor core that way, keys are loaded once for the
+// group, and a causal tile spans few tokens, so that its diagonal wastes
+// little.
+//
+// One CTA per SM, 640 threads, two streams of scores, each with its own S/P
 // and O accumulators in tensor memory (S_t and P_t at columns 128 t, O_t at
 // 256 + 128 t), so that the tensor core works on one stream while the
 // softmax of the other runs:
-//   pair form   stream t is the 128-row tile t of 256 rows; both read every
-//               key block.  For prompts and large trees.
-//   single form both streams are the same 128 rows, stream t reads the key
-//               blocks of parity t, and the two are merged at the end.  For
-//               single tokens and small trees, which are bound by reading the
-//               cache.
+//   pair form   stream t is tile t of two; both read every key block.  For
+//               prompts and large trees.
+//   single form both streams are the same tile, stream t reads the key blocks
+//               of parity t, and the two are merged at the end.  For trees of
+//               65 to 128 rows.
 // Warps:
-//   warp 0       TMA: key and value blocks of 128 keys into two rings, by one
-//                box per block (packed) or one per page part (paged).
-//   warp 1       TMEM owner and MMA issuer: per step O_t += P_t V of the
+//   0, 18        key and value loads: blocks of 128 keys into two rings, one
+//                TMA box per block (packed) or one per page part (paged).
+//   1            TMEM owner and MMA issuer: per step O_t += P_t V of the
 //                stream's previous block, then S_t = Q_t K^T of its next one
 //                (over the columns of that P_t; the MMAs run in order).
-//   warps 2..9   softmax of stream 0, warps 10..17 of stream 1: two threads
-//                per row with 64 of a block's 128 scores each.  They swap
-//                their block maxima through shared memory behind a barrier of
-//                their two warps, keep the running maximum (rescaling O_t in
-//                TMEM only when it grows by more than 2^8: a stale maximum
-//                cancels in O / l) and write P = exp2(scale log2e s - m) over
-//                S_t in parts, each announced to the MMA warp on its own.
+//   2..9, 10..17 softmax of stream 0 and 1: two threads per row with 64 of a
+//                block's 128 scores each.  They swap their block maxima
+//                through shared memory behind a barrier of their two warps,
+//                keep the running maximum (rescaling O_t in TMEM only when it
+//                grows by more than 2^8: a stale maximum cancels in O / l) and
+//                write P = exp2(scale log2e s - m) over S_t in parts, each
+//                announced to the MMA warp on its own.
+//   19           scheduler: finds the next piece of work, hands it to the
+//                others through a small ring, and loads its Q by TMA as soon
+//                as the last scores of the piece before are done.  A piece
+//                used to cost 16000 cycles beyond its blocks (Q loaded row by
+//                row 7900 of them); now its start overlaps the end of the last.
 //
-// Work.  Prompts: one CTA per (256 rows, key head), the tiles with the most
-// keys first.  Cache: the key blocks of all (sequence, key head, row tile)
-// items form one line that is cut into equal shares, one per CTA, so uneven
-// lengths and few long sequences fill the GPU alike; an item that is cut
-// leaves its parts (O, m, l in fp32) in the workspace and
-// attention_join_kernel adds them up in order.
+// Work.  Prompts: a grid of one block per (tile pair, head group), the tiles
+// with the most keys first; a CTA that is done takes over the next block that
+// has not started (cluster launch control).  Cache: the key blocks of all
+// (sequence, head group, tile) items form one line that is cut into equal
+// shares, one per CTA, so uneven lengths and few long sequences fill the GPU
+// alike; an item that is cut leaves its parts (O, m, l in fp32) in the
+// workspace and attention_join_kernel adds them up in order.
 #pragma once
 #include <type_traits>
 
@@ -52,7 +60,7 @@ namespace akili {
 
 constexpr int kSvRows = 128;  // rows of a tile
 constexpr int kSvKeys = 128;  // keys of a block
-constexpr int kSvThreads = 64 + 512;
+constexpr int kSvThreads = 640;
 constexpr int kSvJoinThreads = 256;
 constexpr int kSvJoinSplit = 4;  // blocks that share the rows of a cut item
 
@@ -67,9 +75,13 @@ struct ServingArgs {
   const unsigned int* mask;
   float* parts;  // paged keys: O, m and l of cut items
   int q_heads, kv_heads, group, head_dim, batch, total_q, total_k, causal;
+  int pack;         // heads of a token in one tile; the head groups are q_heads / pack
+  int head_groups;  // q_heads / pack
+  int groups_per_kv;
+  int tile_tokens;  // of a 128-row tile: 128 / pack
   int num_pages, page_size, max_pages, mask_words;
   int box_rows;     // paged keys: rows of a TMA box, a divisor of page_size
-  int chunk_heads;  // packed keys: key heads that are scheduled together
+  int chunk_heads;  // packed keys: head groups that are scheduled together
   float scale_log2;
   long long q_st[2], o_st[2];
   long long table_stride, mask_stride;
@@ -104,79 +116,63 @@ __device__ __forceinline__ SvSeq sv_sequence(const ServingArgs& a, int b, bool* 
   return s;
 }
 
-// A run of key blocks of one (sequence, key head, row tile).
+// A run of key blocks of one (sequence, head group, tile).
 struct SvPiece {
   SvSeq s;
-  int b, hk;
-  int row0, rows;  // first row of the tile(s), rows of the (sequence, key head)
-  int kb;          // first key block
-  int n[2];        // blocks of each stream
-  int loads;       // blocks loaded
-  int part;        // slot of the workspace, or -1: the whole item
+  int b, hk, tile;
+  int kb, loads;  // first key block, blocks
+  int part;       // slot of the workspace, or -1: the whole item
 };
 
-// Keys that some row of [row0, row0 + 128) may see.
-template <bool kPaged>
-__device__ __forceinline__ int sv_key_end(const ServingArgs& a, const SvSeq& s, int row0, int rows) {
-  if (row0 >= rows) return 0;
-  const bool chain = kPaged ? a.mask == nullptr : a.causal != 0;
-  if (!chain) return s.m;
-  const int last = (min(rows, row0 + kSvRows) - 1) / a.group;
-  return max(min(s.m, s.sure + last + 1), 0);
-}
-
-template <bool kPaged, bool kPair>
-__device__ __forceinline__ void sv_streams(const ServingArgs& a, SvPiece& p, int ke) {
-  if constexpr (kPair) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int end = (sv_key_end<kPaged>(a, p.s, p.row0 + t * kSvRows, p.rows) + kSvKeys - 1) / kSvKeys;
-      p.n[t] = max(min(end, ke) - p.kb, 0);
-    }
-    p.loads = max(p.n[0], p.n[1]);
-  } else {
-    p.loads = ke - p.kb;
-    p.n[0] = (p.loads + 1) >> 1;
-    p.n[1] = p.loads >> 1;
-  }
-}
-
-// A CTA's share of the line of key blocks; every role walks it by itself.
-// kTileRows: rows of an item (16 to 256).
+// A CTA's share of the line of key blocks.  kTileRows: rows of an item, 128
+// or 256 of the row forms, 16 to 64 of the few-row form (whose tiles hold
+// consecutive rows and need not start at a token).
 template <int kTileRows>
 struct SvWalk {
   long long pos, begin, end, off;  // off: position within sequence b
   int b;
   SvSeq s;
-  int rows, tiles, blocks;
+  int tiles, blocks;
   long long size;
 
-  __device__ __forceinline__ void load(const ServingArgs& a) {
-    bool clamped;
-    s = sv_sequence<true>(a, b, &clamped);
-    rows = s.n * a.group;
-    tiles = (rows + kTileRows - 1) / kTileRows;
+  __device__ __forceinline__ void load(const ServingArgs& a, bool* clamped) {
+    s = sv_sequence<true>(a, b, clamped);
+    if constexpr (kTileRows >= kSvRows) {
+      const int per = (kTileRows / kSvRows) * a.tile_tokens;
+      tiles = (s.n + per - 1) / per;
+    } else {
+      tiles = (s.n * a.group + kTileRows - 1) / kTileRows;
+    }
     blocks = (s.m + kSvKeys - 1) / kSvKeys;
-    size = static_cast<long long>(a.kv_heads) * tiles * blocks;
+    size = static_cast<long long>(a.head_groups) * tiles * blocks;
   }
   __device__ __forceinline__ bool next(const ServingArgs& a, int cta, SvPiece& p) {
     if (pos >= end) return false;
     while (off >= size) {
       off -= size;
       if (++b >= a.batch) return false;
-      load(a);
+      bool clamped;
+      load(a, &clamped);
     }
-    const long long item = off / blocks;
-    const int kb = static_cast<int>(off - item * blocks);
+    long long item;
+    int kb;
+    if ((off >> 32) == 0) {  // (a 64-bit division costs some 100 cycles more)
+      const uint32_t i = static_cast<uint32_t>(off) / static_cast<uint32_t>(blocks);
+      item = i;
+      kb = static_cast<int>(static_cast<uint32_t>(off) - i * static_cast<uint32_t>(blocks));
+      p.hk = static_cast<int>(i / static_cast<uint32_t>(tiles));
+    } else {
+      item = off / blocks;
+      kb = static_cast<int>(off - item * blocks);
+      p.hk = static_cast<int>(item / tiles);
+    }
     const int take = static_cast<int>(min(static_cast<long long>(blocks - kb), end - pos));
     p.s = s;
     p.b = b;
-    p.hk = static_cast<int>(item / tiles);
-    p.row0 = static_cast<int>(item - static_cast<long long>(p.hk) * tiles) * kTileRows;
-    p.rows = rows;
+    p.tile = static_cast<int>(item - static_cast<long long>(p.hk) * tiles);
     p.kb = kb;
+    p.loads = take;
     p.part = take == blocks ? -1 : 2 * cta + (pos == begin ? 0 : 1);
-    sv_streams<true, kTileRows == 2 * kSvRows>(a, p, kb + take);
     pos += take;
     off += take;
     return true;
@@ -204,12 +200,9 @@ __device__ __forceinline__ long long sv_line_blocks(const ServingArgs& a, int b,
   if (b >= a.batch) return 0;
   SvWalk<kTileRows> w;
   w.b = b;
-  w.load(a);
-  if (record) {
-    bool clamped;
-    sv_sequence<true>(a, b, &clamped);
-    if (clamped) record_bad_index();
-  }
+  bool clamped;
+  w.load(a, &clamped);
+  if (record && clamped) record_bad_index();
   return w.size;
 }
 
@@ -218,8 +211,9 @@ template <int kTileRows>
 __device__ __forceinline__ bool sv_share(const ServingArgs& a, int cta, int ctas, SvWalk<kTileRows>& w,
                                          long long* quota_out, long long* total_out) {
   const int lane = threadIdx.x & 31;
-  long long total = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 32) total += sv_line_blocks<kTileRows>(a, b0 + lane, cta == 0);
+  const long long first = sv_line_blocks<kTileRows>(a, lane, cta == 0);
+  long long total = first;
+  for (int b0 = 32; b0 < a.batch; b0 += 32) total += sv_line_blocks<kTileRows>(a, b0 + lane, cta == 0);
   total = warp_sum(total);
   const long long quota = (total + ctas - 1) / ctas;
   *quota_out = quota;
@@ -229,14 +223,15 @@ __device__ __forceinline__ bool sv_share(const ServingArgs& a, int cta, int ctas
   if (w.begin >= total) return false;
   long long before = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
-    const long long mine = sv_line_blocks<kTileRows>(a, b0 + lane, false);
+    const long long mine = b0 == 0 ? first : sv_line_blocks<kTileRows>(a, b0 + lane, false);
     const long long upto = before + warp_scan(mine);
     const unsigned hit = __ballot_sync(0xffffffffu, upto > w.begin);
     if (hit) {
       const int at = __ffs(hit) - 1;
       w.b = b0 + at;
       w.off = w.begin - __shfl_sync(0xffffffffu, upto - mine, at);
-      w.load(a);
+      bool clamped;
+      w.load(a, &clamped);
       return true;
     }
     before = __shfl_sync(0xffffffffu, upto, 31);
@@ -244,52 +239,61 @@ __device__ __forceinline__ bool sv_share(const ServingArgs& a, int cta, int ctas
   return false;
 }
 
-// Prompts: block `id` of the grid -> (sequence, key head, 256-row tile), one
-// warp; false past the last.  chunk_heads key heads of all sequences are taken
-// together (their keys and values fit in L2 then), within them the tiles
-// level by level from the last (the one with the most keys under a causal
-// mask) to the first, so that the longest start earliest.
+// Prompts: block `id` of the grid -> (sequence, head group, tile pair), one
+// warp; false past the last.  chunk_heads head groups of all sequences are
+// taken together (their keys and values fit in L2 then), within them the tile
+// pairs level by level from the last (the one with the most keys under a
+// causal mask) to the first, so that the longest start earliest.
 __device__ __forceinline__ int sv_levels(const ServingArgs& a, int b) {
   if (b >= a.batch) return 0;
-  bool clamped;
-  return (sv_sequence<false>(a, b, &clamped).n * a.group + 2 * kSvRows - 1) / (2 * kSvRows);
+  const int q0 = min(max(a.cu_q[b], 0), a.total_q);
+  const int n = min(max(a.cu_q[b + 1], q0), a.total_q) - q0;
+  return (n + 2 * a.tile_tokens - 1) / (2 * a.tile_tokens);
 }
-__device__ __forceinline__ bool sv_prompt_tile(const ServingArgs& a, long long id, int* b_out, int* hk, int* level) {
-  const int lane = threadIdx.x & 31;
-  auto at_least = [&](int l) {  // tiles of level l and above
-    long long c = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += 32) c += max(sv_levels(a, b0 + lane) - l, 0);
+struct SvPromptLine {
+  int mine;         // levels of sequence `lane`
+  int top;          // most levels of any sequence
+  long long tiles;  // tile pairs of a head group
+  __device__ __forceinline__ long long at_least(const ServingArgs& a, int l) const {  // tile pairs of level l and above
+    long long c = max(mine - l, 0);
+    for (int b0 = 32; b0 < a.batch; b0 += 32) c += max(sv_levels(a, b0 + static_cast<int>(lane_id())) - l, 0);
     return warp_sum(c);
-  };
-  int top = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 32) top = max(top, sv_levels(a, b0 + lane));
-  top = __reduce_max_sync(0xffffffffu, top);
-  const long long tiles = at_least(0);
-  if (id >= tiles * a.kv_heads) return false;
-  const long long chunk = id / (tiles * a.chunk_heads);
-  const long long rem = id - chunk * tiles * a.chunk_heads;
-  const int heads = min(a.chunk_heads, a.kv_heads - static_cast<int>(chunk) * a.chunk_heads);
-  const long long x = rem / heads;
-  *hk = static_cast<int>(chunk) * a.chunk_heads + static_cast<int>(rem - x * heads);
-  int lo = 0, hi = top - 1;  // the last level with more than x tiles at or above it
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (at_least(mid) > x) lo = mid;
-    else hi = mid - 1;
   }
-  *level = lo;
-  long long left = x - at_least(lo + 1);
-  for (int b0 = 0; b0 < a.batch; b0 += 32) {
-    const unsigned on = __ballot_sync(0xffffffffu, sv_levels(a, b0 + lane) > lo);
-    const int c = __popc(on);
-    if (left < c) {
-      *b_out = b0 + __fns(on, 0, static_cast<int>(left) + 1);
-      return true;
+  __device__ __forceinline__ void load(const ServingArgs& a) {
+    mine = sv_levels(a, static_cast<int>(lane_id()));
+    top = mine;
+    for (int b0 = 32; b0 < a.batch; b0 += 32) top = max(top, sv_levels(a, b0 + static_cast<int>(lane_id())));
+    top = __reduce_max_sync(0xffffffffu, top);
+    tiles = at_least(a, 0);
+  }
+  __device__ __forceinline__ bool find(const ServingArgs& a, long long id, int* b_out, int* hk, int* level) const {
+    if (id >= tiles * a.head_groups) return false;
+    const long long chunk = id / (tiles * a.chunk_heads);
+    const long long rem = id - chunk * tiles * a.chunk_heads;
+    const int heads = min(a.chunk_heads, a.head_groups - static_cast<int>(chunk) * a.chunk_heads);
+    const long long x = rem / heads;
+    *hk = static_cast<int>(chunk) * a.chunk_heads + static_cast<int>(rem - x * heads);
+    int lo = 0, hi = top - 1;  // the last level with more than x tile pairs at or above it
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (at_least(a, mid) > x) lo = mid;
+      else hi = mid - 1;
     }
-    left -= c;
+    *level = lo;
+    long long left = x - at_least(a, lo + 1);
+    for (int b0 = 0; b0 < a.batch; b0 += 32) {
+      const int levels = b0 == 0 ? mine : sv_levels(a, b0 + static_cast<int>(lane_id()));
+      const unsigned on = __ballot_sync(0xffffffffu, levels > lo);
+      const int c = __popc(on);
+      if (left < c) {
+        *b_out = b0 + __fns(on, 0, static_cast<int>(left) + 1);
+        return true;
+      }
+      left -= c;
+    }
+    return false;
   }
-  return false;
-}
+};
 
 // ---------------------------------------------------------- shared memory --
 template <int DP, bool kPair>
@@ -308,21 +312,31 @@ struct SvSmem {
   static_assert(kBytes <= 232448, "227 KB of shared memory per CTA");
 };
 
+// A piece as the scheduler hands it out.
+struct SvTask {
+  int q0, n, k0, m, sure;  // of the sequence
+  int b, hk, tok0;         // sequence, head group, first token of the tile(s)
+  int kb, loads;           // first key block, blocks loaded; loads < 0: no more work
+  int blocks[2];           // blocks of each stream
+  int part;
+  int pad[3];
+};
+constexpr int kSvTasks = 4;
+
 template <int kStages>
 struct SvControl {
-  uint64_t q_full[2];  // pair form: of each tile; single form: the first
+  uint64_t task_full[kSvTasks], task_empty[kSvTasks];
+  uint64_t q_full[2], q_empty[2];  // pair form: of each tile; single form: the first
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
   uint64_t s_full[2], o_done[2];
   uint64_t p_part[4][2];
-  uint64_t drain;
+  uint64_t drain, cancel;
+  uint4 cancelled;  // the answer to a request for a block that has not started
   uint32_t tmem;
-  int work;                   // 0: nothing to do
-  int b, hk, level;           // prompts
-  int pad;
-  long long begin, end, off;  // cache
   // a wait that gave up, for the threads that the next barrier joins: [pair of warps][parity], [quad][parity]
   volatile int pair_abort[8][2];
   volatile int quad_abort[4][2];
+  SvTask task[kSvTasks];
 };
 
 template <typename T>
@@ -348,6 +362,64 @@ __device__ __forceinline__ void tma_load_4d_warp(uint32_t dst, const CUtensorMap
       : "memory");
 }
 
+// Ask for a block of this grid that has not started: its index, or that there
+// is none, arrives in `answer` (16 bytes counted on `bar`).
+__device__ __forceinline__ void request_block(uint4* answer, uint64_t* bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+          smem_u32(answer)),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ bool answered_block(const uint4* answer, uint32_t* index) {
+  uint32_t ok, x;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 h, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+      : "=r"(ok), "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  *index = x;
+  return ok != 0;
+}
+
+// Executed by the whole (converged) warp, as tma_load_4d_warp.
+__device__ __forceinline__ void tma_load_3d_warp(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int y,
+                                                 int z) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+      "[%2];\n\t}" ::"r"(dst),
+      "l"(m), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+// 4 x 4 transpose of 16-byte units between four neighbouring lanes: lane i
+// gives its unit j to lane j as unit i.
+__device__ __forceinline__ void exchange_units(uint32_t (&u)[4][4]) {
+  const uint32_t lane = lane_id();
+#pragma unroll
+  for (int b = 1; b <= 2; b <<= 1) {
+    const bool upper = (lane & b) != 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i & b) continue;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t send = upper ? u[i][w] : u[i | b][w];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, send, b);
+        if (upper) u[i][w] = got;
+        else u[i | b][w] = got;
+      }
+    }
+  }
+}
+
 // Bits [off, off + 64) of a mask row of `words` words; outside it 0.
 __device__ __forceinline__ uint64_t mask_window(const unsigned int* row, int words, int off) {
   const int w = off >> 5, sh = off & 31;
@@ -360,8 +432,8 @@ __device__ __forceinline__ uint64_t mask_window(const unsigned int* row, int wor
 // ----------------------------------------------------------------- kernel --
 template <int DP, typename T, bool kPaged, bool kPair>
 __global__ void __maxnreg__(96)
-    serving_attention_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                             const __grid_constant__ ServingArgs a) {
+    serving_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                             const __grid_constant__ CUtensorMap tmV, const __grid_constant__ ServingArgs a) {
   using L = SvSmem<DP, kPair>;
   constexpr int kTileRows = (kPair ? 2 : 1) * kSvRows;
   constexpr int kStages = L::kStages;
@@ -379,44 +451,20 @@ __global__ void __maxnreg__(96)
   uint8_t* sV = smem + L::kVOff;
   float* xchg = reinterpret_cast<float*>(smem + L::kXOff);
   auto* ctl = reinterpret_cast<SvControl<kStages>*>(smem + L::kCtlOff);
-  static_assert(sizeof(SvControl<kStages>) <= 1024, "control block");
+  static_assert(sizeof(SvControl<kStages>) <= L::kBytes - L::kCtlOff, "control block");
 
   const uint32_t warp = warp_id();
   const uint32_t lane = lane_id();
-  const int cta = blockIdx.x;
   if constexpr (kPaged) griddep_launch_dependents();
 
-  if (warp == 0) {
-    bool work;
-    if constexpr (kPaged) {
-      SvWalk<kTileRows> w;
-      long long quota, total;
-      work = sv_share<kTileRows>(a, cta, gridDim.x, w, &quota, &total);
-      if (lane == 0 && work) {
-        ctl->b = w.b;
-        ctl->begin = w.begin;
-        ctl->end = w.end;
-        ctl->off = w.off;
-      }
-    } else {
-      int b = 0, hk = 0, level = 0;
-      work = sv_prompt_tile(a, cta, &b, &hk, &level);
-      if (lane == 0) {
-        ctl->b = b;
-        ctl->hk = hk;
-        ctl->level = level;
-      }
-    }
-    if (lane == 0) {
-      ctl->work = work && (smem_u32(smem) & 1023) == 0;
-      tma_prefetch_desc(&tmK);
-      tma_prefetch_desc(&tmV);
-    }
-  } else if (warp == 1) {
+  if (warp == 1) {
     tmem_alloc(&ctl->tmem, 512);
     tmem_relinquish();
   } else if (warp == 2 && lane == 0) {
-    for (int t = 0; t < 2; ++t) mbar_init(&ctl->q_full[t], kPair ? 8 : 16);  // one arrive per softmax warp
+    for (int i = 0; i < kSvTasks; ++i) {
+      mbar_init(&ctl->task_full[i], 1);
+      mbar_init(&ctl->task_empty[i], 19);  // every other warp
+    }
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&ctl->k_full[s], 1);
       mbar_init(&ctl->k_empty[s], 1);
@@ -424,110 +472,228 @@ __global__ void __maxnreg__(96)
       mbar_init(&ctl->v_empty[s], 1);
     }
     for (int t = 0; t < 2; ++t) {
+      mbar_init(&ctl->q_full[t], 1);
+      mbar_init(&ctl->q_empty[t], 1);
       mbar_init(&ctl->s_full[t], 1);
       mbar_init(&ctl->o_done[t], 1);
       for (int p = 0; p < kParts; ++p) mbar_init(&ctl->p_part[p][t], 8);  // one arrive per softmax warp
     }
     mbar_init(&ctl->drain, 1);
+    mbar_init(&ctl->cancel, 1);
     for (int i = 0; i < 16; ++i) ctl->pair_abort[i >> 1][i & 1] = 0;
     for (int i = 0; i < 8; ++i) ctl->quad_abort[i >> 1][i & 1] = 0;
     fence_mbar_init();
+  } else if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
   }
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ctl->tmem;
-  const bool work = ctl->work != 0;
 
-  // The pieces of this CTA: one tile (prompts) or a share of the line (cache).
-  SvWalk<kTileRows> walk;
-  int pieces = 0;
-  if constexpr (kPaged) {
-    if (work) {
-      walk.begin = walk.pos = ctl->begin;
-      walk.end = ctl->end;
-      walk.off = ctl->off;
-      walk.b = ctl->b;
-      walk.load(a);
-    }
-  }
-  auto next = [&](SvPiece& p) -> bool {
-    if (!work) return false;
-    if constexpr (kPaged) {
-      return walk.next(a, cta, p);
-    } else {
-      if (pieces++) return false;
-      bool clamped;
-      p.b = ctl->b;
-      p.hk = ctl->hk;
-      p.s = sv_sequence<false>(a, p.b, &clamped);
-      p.rows = p.s.n * a.group;
-      p.row0 = ctl->level * (2 * kSvRows);
-      p.kb = 0;
-      p.part = -1;
-      sv_streams<false, kPair>(a, p, INT32_MAX);
-      return true;
-    }
+  uint32_t n_task = 0;  // pieces taken so far
+  // The next piece for a worker warp; nullptr: no more work, or a wait gave up (*ok false).
+  auto take_task = [&](bool* ok) -> const SvTask* {
+    const uint32_t slot = n_task % kSvTasks;
+    *ok = __all_sync(0xffffffffu, mbar_wait(&ctl->task_full[slot], (n_task / kSvTasks) & 1, kSiteProducerEmpty));
+    const SvTask* t = &ctl->task[slot];
+    if (!*ok || t->loads < 0) return nullptr;
+    ++n_task;
+    return t;
+  };
+  // ... and done with it (its fields are not read again).
+  auto drop_task = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ctl->task_empty[(n_task - 1) % kSvTasks]);
   };
 
-  SvPiece pc;
-  if (warp == 0) {
-    // ------------------------------------------------------------ loads
-    uint32_t count = 0;  // blocks issued to either ring
+  if (warp == 19) {
+    // --------------------------------------------------------------- schedule
+    bool ok = (smem_u32(smem) & 1023) == 0;
+    uint32_t count = 0;            // pieces handed out
+    uint32_t q_used[2] = {0, 0};   // loads of each Q tile
+    uint32_t asked = 0;            // requests for further blocks
+    SvPromptLine line;
+    SvWalk<kTileRows> walk;
+    bool more = ok;
+    if constexpr (kPaged) {
+      long long quota, total;
+      if (ok) more = sv_share<kTileRows>(a, blockIdx.x, gridDim.x, walk, &quota, &total);
+    } else {
+      line.load(a);
+    }
+    uint32_t id = blockIdx.x;
+    while (ok) {
+      SvPiece p;
+      if constexpr (kPaged) {
+        more = more && walk.next(a, blockIdx.x, p);
+      } else {
+        if (count > 0) {
+          // the block that was asked for when the last piece was handed out
+          ok = __all_sync(0xffffffffu, mbar_wait(&ctl->cancel, (asked - 1) & 1, kSiteProducerEmpty));
+          if (!ok) break;
+          more = answered_block(&ctl->cancelled, &id);
+          fence_async_shared();  // read before the next answer is written
+          __syncwarp();
+        }
+        p.kb = 0;
+        p.part = -1;
+        more = more && line.find(a, id, &p.b, &p.hk, &p.tile);
+        if (more) {
+          bool clamped;
+          p.s = sv_sequence<false>(a, p.b, &clamped);
+          if (lane == 0) {
+            mbar_expect_tx(&ctl->cancel, 16);
+            request_block(&ctl->cancelled, &ctl->cancel);
+          }
+          ++asked;
+        }
+      }
+      const uint32_t slot = count % kSvTasks;
+      if (count >= kSvTasks)
+        ok = __all_sync(0xffffffffu, mbar_wait(&ctl->task_empty[slot], (count / kSvTasks - 1) & 1, kSiteProducerEmpty));
+      if (!ok) break;
+      SvTask* t = &ctl->task[slot];
+      if (!more) {
+        if (lane == 0) {
+          t->loads = -1;
+          mbar_arrive(&ctl->task_full[slot]);
+        }
+        break;
+      }
+      const int tok0 = p.tile * (kPair ? 2 : 1) * a.tile_tokens;
+      int n[2], loads;
+      if constexpr (kPair) {
+        // blocks that some row of each tile sees
+        const int ke = kPaged ? p.kb + p.loads : INT32_MAX;
+        const bool chain = kPaged ? a.mask == nullptr : a.causal != 0;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const int first = tok0 + s * a.tile_tokens;
+          int keys = 0;
+          if (first < p.s.n)
+            keys = chain ? max(min(p.s.m, p.s.sure + min(p.s.n, first + a.tile_tokens)), 0) : p.s.m;
+          n[s] = max(min((keys + kSvKeys - 1) / kSvKeys, ke) - p.kb, 0);
+        }
+        loads = max(n[0], n[1]);
+      } else {
+        loads = p.loads;
+        n[0] = (loads + 1) >> 1;
+        n[1] = loads >> 1;
+      }
+      if (lane == 0) {
+        t->q0 = p.s.q0;
+        t->n = p.s.n;
+        t->k0 = p.s.k0;
+        t->m = p.s.m;
+        t->sure = p.s.sure;
+        t->b = p.b;
+        t->hk = p.hk;
+        t->tok0 = tok0;
+        t->kb = p.kb;
+        t->loads = loads;
+        t->blocks[0] = n[0];
+        t->blocks[1] = n[1];
+        t->part = p.part;
+        mbar_arrive(&ctl->task_full[slot]);
+      }
+      __syncwarp();
+      ++count;
+      // Q: tile_tokens x pack rows of each tile (the last rows of a tile that
+      // pack does not divide, and rows past the sequence, are nobody's)
+#pragma unroll
+      for (int s = 0; s < (kPair ? 2 : 1); ++s) {
+        if (!ok || (kPair ? n[s] : loads) == 0) continue;
+        if (q_used[s] > 0)
+          ok = __all_sync(0xffffffffu, mbar_wait(&ctl->q_empty[s], (q_used[s] - 1) & 1, kSiteFlashQ));
+        if (!ok) continue;
+        ++q_used[s];
+        if (lane == 0) mbar_expect_tx(&ctl->q_full[s], a.tile_tokens * a.pack * 128 * kChunks);
+        __syncwarp();
+        for (int c = 0; c < kChunks; ++c)
+          tma_load_3d_warp(smem_u32(sQ + s * L::kQ + c * 16384), &tmQ, smem_u32(&ctl->q_full[s]), c * 64,
+                           p.hk * a.pack, p.s.q0 + tok0 + s * a.tile_tokens);
+      }
+    }
+    // What was asked for arrives before the CTA ends; so do the Q tiles (the MMA
+    // warp waits for them, or, if a wait gave up, this one does).
+    if constexpr (!kPaged)
+      if (!ok && asked > 0) mbar_wait(&ctl->cancel, (asked - 1) & 1, kSiteDrain);
+    if (!ok)
+      for (int s = 0; s < 2; ++s)
+        if (q_used[s] > 0) mbar_wait(&ctl->q_full[s], (q_used[s] - 1) & 1, kSiteDrain);
+    __syncwarp();
+  } else if (warp == 0 || warp == 18) {
+    // ------------------------------------------------------ key / value loads
+    const bool is_v = warp == 18;
+    const CUtensorMap* tm = is_v ? &tmV : &tmK;
+    uint8_t* ring = is_v ? sV : sK;
+    uint64_t* full = is_v ? ctl->v_full : ctl->k_full;
+    uint64_t* empty = is_v ? ctl->v_empty : ctl->k_empty;
+    int st = 0;
+    uint32_t round = 0, issued = 0;
     bool ok = true;
-    while (ok && next(pc)) {
-      for (int j = 0; j < pc.loads && ok; ++j, ++count) {
-        const int st = count % kStages;
-        const uint32_t ph = (count / kStages) & 1;
-        const int key0 = (pc.kb + j) * kSvKeys;
-        uint32_t bytes = L::kKV;
-        int page = 0, boxes = 0;
-        const bool mine = lane == 0;
+    while (const SvTask* t = take_task(&ok)) {
+      const int loads = t->loads, kb = t->kb, m = t->m, k0 = t->k0, b = t->b;
+      const int kv_head = t->hk / a.groups_per_kv;
+      drop_task();
+      const int* table = kPaged ? a.page_table + b * a.table_stride : nullptr;
+      // lane x looks up the page of box x (box_rows keys), a block ahead
+      auto lookup = [&](int j) -> int {
+        int page = 0;
         if constexpr (kPaged) {
-          // lane b looks up the page of box b (box_rows keys)
-          boxes = (min(kSvKeys, pc.s.m - key0) + a.box_rows - 1) / a.box_rows;
-          bytes = static_cast<uint32_t>(boxes * a.box_rows * 128 * kChunks);
-          if (static_cast<int>(lane) < boxes) {
-            const int key = key0 + static_cast<int>(lane) * a.box_rows;
-            page = a.page_table[pc.b * a.table_stride + key / a.page_size];
+          const int in = static_cast<int>(lane) * a.box_rows;
+          const int key = (kb + j) * kSvKeys + in;
+          if (j < loads && in < kSvKeys && key < m) {
+            page = table[key / a.page_size];
             if (page < 0 || page >= a.num_pages) {  // outside the tensor: TMA fills zeros
               record_bad_index();
               page = -1;
             }
           }
         }
-        auto load = [&](const CUtensorMap& tm, uint8_t* ring, uint64_t* full, uint64_t* empty) {
-          if (count >= kStages) ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], ph ^ 1, kSiteFlashFree));
-          if (!ok) return;
-          if (lane == 0) mbar_expect_tx(&full[st], bytes);
+        return page;
+      };
+      int page = lookup(0);
+      for (int j = 0; j < loads; ++j) {
+        const int key0 = (kb + j) * kSvKeys;
+        const int ahead = lookup(j + 1);
+        if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], (round - 1) & 1, kSiteFlashFree));
+        if (!ok) break;
+        const uint32_t dst = smem_u32(ring + st * L::kKV), bar = smem_u32(&full[st]);
+        if constexpr (kPaged) {
+          const int boxes = (min(kSvKeys, m - key0) + a.box_rows - 1) / a.box_rows;
+          if (lane == 0) mbar_expect_tx(&full[st], static_cast<uint32_t>(boxes * a.box_rows * 128 * kChunks));
           __syncwarp();
-          if constexpr (kPaged) {
-            const uint32_t dst = smem_u32(ring + st * L::kKV), bar = smem_u32(&full[st]);
-            int in_page = key0 % a.page_size;
+          int in_page = key0 % a.page_size;
 #pragma unroll 4
-            for (int box = 0; box < boxes; ++box) {
-              const int at = __shfl_sync(0xffffffffu, page, box);
-              for (int c = 0; c < kChunks; ++c)
-                tma_load_4d_warp(dst + c * 16384 + box * a.box_rows * 128, &tm, bar, c * 64, in_page, pc.hk, at);
-              in_page += a.box_rows;
-              if (in_page == a.page_size) in_page = 0;
-            }
-          } else {
-            if (mine)
-              for (int c = 0; c < kChunks; ++c)
-                tma_load_3d(ring + st * L::kKV + c * 16384, &tm, &full[st], c * 64, pc.hk, pc.s.k0 + key0);
+          for (int box = 0; box < boxes; ++box) {
+            const int at = __shfl_sync(0xffffffffu, page, box);
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c)
+              tma_load_4d_warp(dst + c * 16384 + box * a.box_rows * 128, tm, bar, c * 64, in_page, kv_head, at);
+            in_page += a.box_rows;
+            if (in_page == a.page_size) in_page = 0;
           }
-        };
-        load(tmK, sK, ctl->k_full, ctl->k_empty);
-        if (ok) load(tmV, sV, ctl->v_full, ctl->v_empty);
+        } else {
+          if (lane == 0) mbar_expect_tx(&full[st], L::kKV);
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) tma_load_3d_warp(dst + c * 16384, tm, bar, c * 64, kv_head, k0 + key0);
+        }
+        ++issued;
+        page = ahead;
+        if (++st == kStages) {
+          st = 0;
+          ++round;
+        }
       }
+      if (!ok) break;
     }
-    if (!ok) {
-      // a wait gave up: the loads in flight end before the CTA does
-      for (uint32_t c = count > kStages ? count - kStages : 0; c < count; ++c) {
-        mbar_wait(&ctl->k_full[c % kStages], (c / kStages) & 1, kSiteDrain);
-        mbar_wait(&ctl->v_full[c % kStages], (c / kStages) & 1, kSiteDrain);
-      }
-    }
+    if (!ok)  // a wait gave up: the loads in flight end before the CTA does
+      for (uint32_t c = issued > kStages ? issued - kStages : 0; c < issued; ++c)
+        mbar_wait(&full[c % kStages], (c / kStages) & 1, kSiteDrain);
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------- MMA
@@ -545,10 +711,9 @@ __global__ void __maxnreg__(96)
       ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, site));
     };
     // Values past the sequence's end may be anything: 0 times them must be 0.
-    auto take_values = [&](int block) {
+    auto take_values = [&](int live) {
       const int st = vc % kStages;
       wait(&ctl->v_full[st], (vc / kStages) & 1, kSiteFlashKV);
-      const int live = pc.s.m - block * kSvKeys;
       if (ok && live < kSvKeys) {
         const uint4 zero = {0, 0, 0, 0};
         for (int c = 0; c < kChunks; ++c)
@@ -591,24 +756,30 @@ __global__ void __maxnreg__(96)
       }
       umma_commit_warp(&ctl->s_full[t]);
     };
-    while (ok && next(pc)) {
-      // (a tile without blocks in this piece is not loaded: its warps go on to the next piece)
-      if (!kPair || pc.n[0] > 0) wait(&ctl->q_full[0], q_cnt[0]++ & 1, kSiteFlashQ);
-      if (kPair && pc.n[1] > 0) wait(&ctl->q_full[1], q_cnt[1]++ & 1, kSiteFlashQ);
+    while (const SvTask* task = take_task(&ok)) {
+      const int loads = task->loads, n0 = task->blocks[0], n1 = task->blocks[1];
+      const int tail = task->m - task->kb * kSvKeys;  // keys from this piece's first block on
+      drop_task();
       if constexpr (kPair) {
-        for (int j = 0; j <= pc.loads && ok; ++j) {
-          if (j < pc.loads) wait(&ctl->k_full[kc % kStages], (kc / kStages) & 1, kSiteFlashKV);
-          if (j >= 1) take_values(pc.kb + j - 1);
+        for (int j = 0; j <= loads && ok; ++j) {
+          if (j < loads) wait(&ctl->k_full[kc % kStages], (kc / kStages) & 1, kSiteFlashKV);
+          if (j >= 1) take_values(tail - (j - 1) * kSvKeys);
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (ok && j >= 1 && j <= pc.n[t]) {
+            const int n = t == 0 ? n0 : n1;
+            if (ok && j >= 1 && j <= n) {
               issue_pv(t, j == 1);
-              if (ok && j == pc.n[t]) umma_commit_warp(&ctl->o_done[t]);
+              if (ok && j == n) umma_commit_warp(&ctl->o_done[t]);
             }
-            if (ok && j < pc.n[t]) issue_s(t);
+            if (ok && j < n) {
+              if (j == 0) wait(&ctl->q_full[t], q_cnt[t]++ & 1, kSiteFlashQ);
+              if (!ok) break;
+              issue_s(t);
+              if (j == n - 1) umma_commit_warp(&ctl->q_empty[t]);
+            }
           }
           if (!ok) break;
-          if (j < pc.loads) {
+          if (j < loads) {
             umma_commit_warp(&ctl->k_empty[kc % kStages]);
             ++kc;
           }
@@ -618,28 +789,31 @@ __global__ void __maxnreg__(96)
           }
         }
       } else {
-        for (int j = 0; j < pc.loads + 2 && ok; ++j) {
+        wait(&ctl->q_full[0], q_cnt[0]++ & 1, kSiteFlashQ);
+        for (int j = 0; j < loads + 2 && ok; ++j) {
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if ((j & 1) != t) continue;
             if (j >= 2) {
-              take_values(pc.kb + j - 2);
+              take_values(tail - (j - 2) * kSvKeys);
               if (ok) issue_pv(t, j == 2 + t);
               if (!ok) break;
               umma_commit_warp(&ctl->v_empty[vc % kStages]);
               ++vc;
-              if (j >= pc.loads) umma_commit_warp(&ctl->o_done[t]);
+              if (j >= loads) umma_commit_warp(&ctl->o_done[t]);
             }
-            if (j < pc.loads) {
+            if (j < loads) {
               wait(&ctl->k_full[kc % kStages], (kc / kStages) & 1, kSiteFlashKV);
               if (!ok) break;
               issue_s(t);
               umma_commit_warp(&ctl->k_empty[kc % kStages]);
+              if (j == loads - 1) umma_commit_warp(&ctl->q_empty[0]);
               ++kc;
             }
           }
         }
       }
+      if (!ok) break;
     }
     umma_commit_warp(&ctl->drain);
     mbar_wait(&ctl->drain, 0, kSiteDrain);
@@ -650,6 +824,8 @@ __global__ void __maxnreg__(96)
     const int half = ((static_cast<int>(warp) - 2) >> 2) & 1;  // of a block's scores
     const int wq = static_cast<int>(warp & 3);                 // TMEM lane quarter
     const int r = wq * 32 + static_cast<int>(lane);            // row of the tile
+    const int row_tok = r / a.pack;                            // its token and head within the tile
+    const int row_head = r - row_tok * a.pack;
     const int pair_id = grp * 4 + wq;
     const uint32_t pair_bar = 1 + pair_id;  // 64 threads: both halves of these rows
     const uint32_t quad_bar = 9 + wq;       // 128 threads: both halves, both streams
@@ -660,49 +836,25 @@ __global__ void __maxnreg__(96)
     uint32_t events = 0;  // barriers of the pair so far, the parity of its abort flags
     uint32_t s_cnt = 0;   // blocks of this stream so far
     uint32_t o_cnt[2] = {0, 0};
-    uint32_t n_piece = 0;
     bool alive = true;
     auto swap_slot = [&](uint32_t ev) {
       return xchg + ((L::kXBufs == 2 ? (ev & 1) * 2 : 0) + grp) * (2 * kSvRows);
     };
-    while (alive && next(pc)) {
+    bool ok = true;
+    while (const SvTask* task = take_task(&ok)) {
+      const uint32_t piece_parity = n_task & 1;
       // ---- this piece's row
-      const int row = pc.row0 + (kPair ? grp * kSvRows : 0) + r;
-      const bool live = row < pc.rows;
-      const int tok = live ? row / a.group : 0;
-      const int head = pc.hk * a.group + (live ? row - tok * a.group : 0);
-      const long long qrow = pc.s.q0 + tok;
+      const int tok = task->tok0 + (kPair ? grp * a.tile_tokens : 0) + row_tok;
+      const bool live = row_tok < a.tile_tokens && tok < task->n;
       const bool tree = kPaged && a.mask != nullptr;
-      int sees = pc.s.m;  // keys 0 .. sees - 1 are visible (and the nodes of the mask row)
-      if (tree) sees = pc.s.sure;
-      else if (kPaged || a.causal) sees = min(pc.s.m, pc.s.sure + tok + 1);
+      int sees = task->m;  // keys 0 .. sees - 1 are visible (and the nodes of the mask row)
+      if (tree) sees = task->sure;
+      else if (kPaged || a.causal) sees = min(task->m, task->sure + tok + 1);
       if (!live) sees = 0;
-      // ---- Q into shared memory (K-major, 128-byte swizzle), zero past the rows and the head
-      if (!kPair || pc.n[grp] > 0) {
-        constexpr int kCols = kPair ? DP / 2 : DP / 4;  // of this thread
-        const int c0 = kPair ? half * kCols : (2 * grp + half) * kCols;
-        const T* src = static_cast<const T*>(a.q) + qrow * a.q_st[0] + head * a.q_st[1];
-        uint4 v[kCols / 8];
-#pragma unroll
-        for (int x = 0; x < kCols / 8; ++x) {
-          v[x] = uint4{0, 0, 0, 0};
-          if (live && c0 + x * 8 < a.head_dim) v[x] = *reinterpret_cast<const uint4*>(src + c0 + x * 8);
-        }
-        uint8_t* dst = sQ + (kPair ? grp * L::kQ : 0) + r * 128;
-#pragma unroll
-        for (int x = 0; x < kCols / 8; ++x) {
-          const int c = (c0 + x * 8) / 8;  // 16-byte column
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * 16384 + (((c & 7) ^ (r & 7)) << 4)) = v[x];
-        }
-        fence_async_shared();
-        tc_fence_before();  // the last piece's O has been read
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->q_full[kPair ? grp : 0]);
-      }
-      float m_use = -INFINITY;
-      float m_true = -INFINITY;  // exact running maximum (m_use may lag it by the rescale threshold)
-      float l = 0.0f;            // this half's share of the row sum
-      const int nblk = pc.n[grp];
+      float m_use = -INFINITY;  // running maximum, exact to the rescale threshold
+      float l = 0.0f;           // this half's share of the row sum
+      const int nblk = task->blocks[grp];
+      const int kv_first = task->kb * kSvKeys + (kPair ? 0 : grp * kSvKeys) + half * 64;
       const bool warp_live = __any_sync(0xffffffffu, live);
       for (int i = 0; i < nblk; ++i, ++s_cnt, ++events) {
         if (!mbar_wait(&ctl->s_full[grp], s_cnt & 1, kSiteFlashS)) ctl->pair_abort[pair_id][events & 1] = 1;
@@ -719,7 +871,7 @@ __global__ void __maxnreg__(96)
           continue;
         }
         tc_fence_after();
-        const int kv0 = (pc.kb + (kPair ? i : 2 * i + grp)) * kSvKeys + half * 64;
+        const int kv0 = kv_first + i * (kPair ? kSvKeys : 2 * kSvKeys);
         float s[64];
         tmem_ld64(tS, s);
         float mx[8];
@@ -732,10 +884,10 @@ __global__ void __maxnreg__(96)
           const int nv = sees - kv0;
           uint64_t vis = nv <= 0 ? 0ull : (1ull << nv) - 1;
           if (tree && live) {
-            const int node = kv0 - pc.s.sure;  // of this half's first key
-            const int nodes = pc.s.m - pc.s.sure;
+            const int node = kv0 - task->sure;  // of this half's first key
+            const int nodes = task->m - task->sure;
             if (node > -64 && node < nodes) {
-              uint64_t bits = mask_window(a.mask + qrow * a.mask_stride, a.mask_words, node);
+              uint64_t bits = mask_window(a.mask + (task->q0 + tok) * a.mask_stride, a.mask_words, node);
               if (nodes - node < 64) bits &= (1ull << (nodes - node)) - 1;
               vis |= bits;
             }
@@ -760,7 +912,6 @@ __global__ void __maxnreg__(96)
           break;
         }
         const float rmax = sl * fmaxf(pmax, other);
-        m_true = fmaxf(m_true, rmax);
         const bool grow = rmax > m_use + 8.0f;
         const float m_new = grow ? rmax : m_use;
         const float alpha = grow ? exp2f(m_use - m_new) : 1.0f;  // 0 on the first block with a visible key
@@ -808,14 +959,12 @@ __global__ void __maxnreg__(96)
       // ---- output.  With the pair form each half of a stream has half of
       // the row's columns; with the single form the row's four threads have a
       // quarter each, of the sum of both streams.
-      float* slot = nullptr;  // [kRows][DP] O, [kRows] m, [kRows] l
-      if (kPaged && pc.part >= 0) slot = a.parts + static_cast<size_t>(pc.part) * kTileRows * (DP + 2);
-      const int prow = (kPair ? grp * kSvRows : 0) + r;
-      T* out = static_cast<T*>(a.o) + qrow * a.o_st[0] + head * a.o_st[1];
-      float w0 = 0.0f, w1 = 0.0f;  // of O_0 and O_1 (pair form: w0 of this stream's)
+      if (kPair && !alive) break;
+      float w0, w1 = 0.0f;  // of O_0 and O_1 (pair form: w0 of this stream's)
       float l_row, m_row;
+      const int part = task->part;
+      const bool whole = !kPaged || part < 0;
       if constexpr (kPair) {
-        if (!alive) break;
         float* xs = swap_slot(events);
         xs[half * kSvRows + r] = l;
         if (nblk > 0 && !mbar_wait(&ctl->o_done[grp], o_cnt[grp] & 1, kSiteFlashPV))
@@ -829,16 +978,16 @@ __global__ void __maxnreg__(96)
         }
         ++events;
         m_row = m_use;
-        w0 = slot != nullptr ? 1.0f : l_row > 0.0f || l_row != l_row ? 1.0f / l_row : 0.0f;
+        w0 = !whole ? 1.0f : l_row != 0.0f ? 1.0f / l_row : 0.0f;
         if (nblk == 0) w0 = 0.0f;
       } else {
-        if (!alive) ctl->quad_abort[wq][n_piece & 1] = 1;
+        if (!alive) ctl->quad_abort[wq][piece_parity] = 1;
         // both streams of this row: m and the two halves' sums
         float* xs = xchg;
         for (int t = 0; t < 2; ++t) {
-          if (pc.n[t] > 0 && !mbar_wait(&ctl->o_done[t], o_cnt[t] & 1, kSiteFlashPV))
-            ctl->quad_abort[wq][n_piece & 1] = 1;
-          if (pc.n[t] > 0) ++o_cnt[t];
+          const int n = task->blocks[t];
+          if (n > 0 && !mbar_wait(&ctl->o_done[t], o_cnt[t] & 1, kSiteFlashPV)) ctl->quad_abort[wq][piece_parity] = 1;
+          if (n > 0) ++o_cnt[t];
         }
         named_bar_sync(quad_bar, 128);  // the last block's exchange has been read
         xs[(grp * 2 + half) * kSvRows + r] = l;
@@ -850,7 +999,7 @@ __global__ void __maxnreg__(96)
         named_bar_sync(quad_bar, 128);
         const float m0 = xs[0 * kSvRows + r], m1 = xs[1 * kSvRows + r];
         named_bar_sync(quad_bar, 128);
-        if (ctl->quad_abort[wq][n_piece & 1]) {
+        if (ctl->quad_abort[wq][piece_parity]) {
           alive = false;
           break;
         }
@@ -859,53 +1008,79 @@ __global__ void __maxnreg__(96)
         w0 = exp2f(m0 - m_sub);  // 0 for a stream that saw nothing
         w1 = exp2f(m1 - m_sub);
         l_row = l0 * w0 + l1 * w1;
-        if (slot == nullptr) {
-          const float inv = l_row > 0.0f || l_row != l_row ? 1.0f / l_row : 0.0f;
+        if (whole) {
+          const float inv = l_row != 0.0f ? 1.0f / l_row : 0.0f;
           w0 *= inv;
           w1 *= inv;
         }
       }
-      ++n_piece;
       tc_fence_after();
       if (warp_live) {
         constexpr int kCols = kPair ? DP / 2 : DP / 4;
         const int c0 = kPair ? half * kCols : (2 * grp + half) * kCols;
-        constexpr int kStep = kCols < 32 ? kCols : 32;
+        const bool on0 = task->blocks[kPair ? grp : 0] > 0;
+        const bool on1 = !kPair && task->blocks[1] > 0;
+        const int head = task->hk * a.pack + row_head;
+        const long long qrow = task->q0 + tok;
+        // parts: [unit of 4 columns][row][4], m, l
+        const int prow = (kPair ? grp * kSvRows : 0) + r;
+        float* slot = whole ? nullptr : a.parts + static_cast<size_t>(part) * kTileRows * (DP + 2);
+        // the rows of this lane's four neighbours, for which it stores one unit of each
+        T* out[4];
+        bool put[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const long long to = __shfl_sync(0xffffffffu, qrow * a.o_st[0] + head * a.o_st[1], (lane & ~3u) + x);
+          put[x] = __shfl_sync(0xffffffffu, static_cast<int>(live), (lane & ~3u) + x) != 0;
+          out[x] = static_cast<T*>(a.o) + to;
+        }
+        constexpr int kStep = 32 < kCols ? 32 : kCols;  // 32 or 16 columns at a time
 #pragma unroll 1
         for (int c = c0; c < c0 + kCols; c += kStep) {
           float o[kStep];
 #pragma unroll
           for (int x = 0; x < kStep; ++x) o[x] = 0.0f;
-#pragma unroll
-          for (int t = 0; t < (kPair ? 1 : 2); ++t) {
-            const int u = kPair ? grp : t;
-            if (pc.n[u] == 0) continue;  // nothing was accumulated there
-            const float w = t == 0 ? w0 : w1;
+          if (on0) {
+            const uint32_t src = tmem + lane_off + kColO + (kPair ? grp : 0) * 128 + c;
 #pragma unroll
             for (int x = 0; x < kStep; x += 8) {
               uint32_t e[8];
-              tmem_ld8(tmem + lane_off + kColO + u * 128 + c + x, e);
+              tmem_ld8(src + x, e);
 #pragma unroll
-              for (int y = 0; y < 8; ++y) o[x + y] += w != 0.0f ? w * __uint_as_float(e[y]) : 0.0f;
+              for (int y = 0; y < 8; ++y) o[x + y] = w0 != 0.0f ? w0 * __uint_as_float(e[y]) : 0.0f;
             }
           }
-          if (!live) continue;
+          if (on1) {
+            const uint32_t src = tmem + lane_off + kColO + 128 + c;
+#pragma unroll
+            for (int x = 0; x < kStep; x += 8) {
+              uint32_t e[8];
+              tmem_ld8(src + x, e);
+#pragma unroll
+              for (int y = 0; y < 8; ++y) o[x + y] += w1 != 0.0f ? w1 * __uint_as_float(e[y]) : 0.0f;
+            }
+          }
           if (slot != nullptr) {
+            if (live)
 #pragma unroll
-            for (int x = 0; x < kStep; x += 4)
-              *reinterpret_cast<float4*>(slot + static_cast<size_t>(prow) * DP + c + x) =
-                  make_float4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+              for (int x = 0; x < kStep; x += 4)
+                *reinterpret_cast<float4*>(slot + (static_cast<size_t>((c + x) / 4) * kTileRows + prow) * 4) =
+                    make_float4(o[x], o[x + 1], o[x + 2], o[x + 3]);
           } else {
+            uint32_t u[4][4];
 #pragma unroll
-            for (int x = 0; x < kStep; x += 8)
-              if (c + x < a.head_dim) {
-                uint4 v;
-                v.x = pack2<T>(o[x], o[x + 1]);
-                v.y = pack2<T>(o[x + 2], o[x + 3]);
-                v.z = pack2<T>(o[x + 4], o[x + 5]);
-                v.w = pack2<T>(o[x + 6], o[x + 7]);
-                *reinterpret_cast<uint4*>(out + c + x) = v;
-              }
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+              for (int w = 0; w < 4; ++w)
+                u[x][w] = x * 8 < kStep ? pack2<T>(o[(x * 8 + 2 * w) % kStep], o[(x * 8 + 2 * w + 1) % kStep]) : 0u;
+            exchange_units(u);
+            // u[x] is now unit lane & 3 of neighbour x's row: 64 bytes in a row per four lanes
+            const int col = c + static_cast<int>(lane & 3) * 8;
+            const bool in = static_cast<int>(lane & 3) * 8 < kStep && col < a.head_dim;
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (in && put[x])
+                *reinterpret_cast<uint4*>(out[x] + col) = make_uint4(u[x][0], u[x][1], u[x][2], u[x][3]);
           }
         }
         if (live && half == 0 && (kPair || grp == 0)) {
@@ -917,6 +1092,8 @@ __global__ void __maxnreg__(96)
           }
         }
       }
+      tc_fence_before();  // O has been read before the next P is announced
+      drop_task();
     }
   }
 
@@ -928,11 +1105,14 @@ __global__ void __maxnreg__(96)
 }
 
 // Adds up the parts of the item that starts in share c = blockIdx.x and goes
-// on past its end, in order: a warp per row, four values of the head per lane.
+// on past its end, in order.
 //   m = max m_p,  o = sum 2^(m_p - m) O_p / sum 2^(m_p - m) l_p
+// Row forms: a thread per (row, four columns), rows along the lanes, as the
+// parts are laid out.  Few-row form (parts row by row): a warp per row.
 template <int DP, typename T, int kTileRows>
 __global__ void __launch_bounds__(kSvJoinThreads) attention_join_kernel(const __grid_constant__ ServingArgs a) {
-  __shared__ int from, parts, slot0, row0, rows, q0, hk;
+  constexpr bool kByRow = kTileRows < kSvRows;
+  __shared__ int from, parts, slot0, first, tokens, q0, hk;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
     SvWalk<kTileRows> w;
@@ -950,8 +1130,8 @@ __global__ void __launch_bounds__(kSvJoinThreads) attention_join_kernel(const __
         from = blockIdx.x;
         parts = static_cast<int>(last) - blockIdx.x + 1;
         slot0 = p.part;
-        row0 = p.row0;
-        rows = p.rows;
+        first = kByRow ? p.tile * kTileRows : p.tile * (kTileRows / kSvRows) * a.tile_tokens;
+        tokens = p.s.n;
         q0 = p.s.q0;
         hk = p.hk;
       }
@@ -960,43 +1140,55 @@ __global__ void __launch_bounds__(kSvJoinThreads) attention_join_kernel(const __
   __syncthreads();
   griddep_wait();  // the parts
   if (parts == 0) return;
-  const int n = min(kTileRows, rows - row0);
   constexpr size_t kSlot = static_cast<size_t>(kTileRows) * (DP + 2);
   auto part = [&](int i) { return a.parts + (i == 0 ? slot0 : 2 * (from + i)) * kSlot; };
-  for (int r = blockIdx.y * (kSvJoinThreads / 32) + warp; r < n; r += gridDim.y * (kSvJoinThreads / 32)) {
+  constexpr size_t kM = static_cast<size_t>(kTileRows) * DP, kL = static_cast<size_t>(kTileRows) * (DP + 1);
+  // row r of the item -> its token and head within the group; false if it is nobody's
+  auto row_of = [&](int r, int* tok, int* head) {
+    if constexpr (kByRow) {
+      const int row = first + r;
+      *tok = row / a.group;
+      *head = row - *tok * a.group;
+      return *tok < tokens;
+    } else {
+      const int in = r % kSvRows, t = in / a.pack;
+      *tok = first + r / kSvRows * a.tile_tokens + t;
+      *head = in - t * a.pack;
+      return t < a.tile_tokens && *tok < tokens;
+    }
+  };
+  constexpr int kUnits = kByRow ? 32 : DP / 4;  // threads of a row
+  const int step = gridDim.y * kSvJoinThreads;
+  for (int x = blockIdx.y * kSvJoinThreads + threadIdx.x; x < kTileRows * kUnits; x += step) {
+    const int r = kByRow ? x / kUnits : x % kTileRows, unit = kByRow ? x % kUnits : x / kTileRows;
+    int tok, head;
+    if (!row_of(r, &tok, &head) || unit * 4 >= a.head_dim) continue;
     float m = -INFINITY;
-    for (int i = lane; i < parts; i += 32) m = fmaxf(m, part(i)[static_cast<size_t>(kTileRows) * DP + r]);
-#pragma unroll
-    for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+    for (int i = 0; i < parts; ++i) m = fmaxf(m, part(i)[kM + r]);
     const float m_sub = m == -INFINITY ? 0.0f : m;
     float o[4] = {}, l = 0.0f;
-    const int d = lane * 4;
-    const bool on = d < a.head_dim;
 #pragma unroll 4
     for (int i = 0; i < parts; ++i) {
       const float* p = part(i);
-      const float w = exp2f(p[static_cast<size_t>(kTileRows) * DP + r] - m_sub);
-      l += w * p[static_cast<size_t>(kTileRows) * (DP + 1) + r];
-      if (on && w != 0.0f) {
-        const float4 v = *reinterpret_cast<const float4*>(p + static_cast<size_t>(r) * DP + d);
+      const float w = exp2f(p[kM + r] - m_sub);
+      l += w * p[kL + r];
+      if (w != 0.0f) {
+        const float4 v = *reinterpret_cast<const float4*>(
+            p + (kByRow ? static_cast<size_t>(r) * DP + unit * 4 : (static_cast<size_t>(unit) * kTileRows + r) * 4));
         o[0] += w * v.x;
         o[1] += w * v.y;
         o[2] += w * v.z;
         o[3] += w * v.w;
       }
     }
-    const int row = row0 + r;
-    const int tok = row / a.group;
-    const int head = hk * a.group + row - tok * a.group;
     const long long qrow = q0 + tok;
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    if (on) {
-      uint2 v;
-      v.x = pack2<T>(o[0] * inv, o[1] * inv);
-      v.y = pack2<T>(o[2] * inv, o[3] * inv);
-      *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + qrow * a.o_st[0] + head * a.o_st[1] + d) = v;
-    }
-    if (a.lse != nullptr && lane == 0) a.lse[qrow * a.q_heads + head] = (m + log2f(l)) * 0.6931471805599453f;
+    const int qh = hk * (kByRow ? a.group : a.pack) + head;
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    uint2 v;
+    v.x = pack2<T>(o[0] * inv, o[1] * inv);
+    v.y = pack2<T>(o[2] * inv, o[3] * inv);
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + qrow * a.o_st[0] + qh * a.o_st[1] + unit * 4) = v;
+    if (a.lse != nullptr && unit == 0) a.lse[qrow * a.q_heads + qh] = (m + log2f(l)) * 0.6931471805599453f;
   }
 }
 

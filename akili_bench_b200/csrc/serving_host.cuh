@@ -256,16 +256,15 @@ float scale_log2_of(float scale, uint32_t d) {
 }
 
 // [d3][d2][d1][d0] tensor of 16-bit values with these strides (elements), box
-// [1][1][box1][64], 128-byte swizzle.  The stride of an axis of one entry is never used.
+// [box3][box2][box1][64], 128-byte swizzle.  The stride of an axis of one entry is never used.
 bool map_heads(CUtensorMap* m, const void* ptr, uint32_t dtype, int rank, const uint64_t (&dim)[4],
-               const int64_t (&stride)[3], int box_axis, uint32_t box) {
+               const int64_t (&stride)[3], const uint32_t (&box)[3]) {
   EncodeTiledFn enc = encode_fn();
   if (!enc) return false;
   cuuint64_t dims[4], strides[3];
-  cuuint32_t boxes[4] = {64, 1, 1, 1}, es[4] = {1, 1, 1, 1};
+  cuuint32_t boxes[4] = {64, box[0], box[1], box[2]}, es[4] = {1, 1, 1, 1};
   for (int i = 0; i < rank; ++i) dims[i] = dim[i];
   for (int i = 0; i + 1 < rank; ++i) strides[i] = dim[i + 1] == 1 ? (dim[0] * 2 + 15) / 16 * 16 : stride[i] * 2;
-  boxes[box_axis] = box;
   return enc(m, dtype == AKILI_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
              const_cast<void*>(ptr), dims, strides, boxes, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -291,20 +290,40 @@ struct SmemGrant {
   }
 };
 
+// Packing of a token's heads into the rows of a 128-row tile.
+void pack_heads(ServingArgs& g) {
+  g.pack = g.group;
+  while (g.pack > kSvRows || g.group % g.pack) --g.pack;
+  g.head_groups = g.q_heads / g.pack;
+  g.groups_per_kv = g.group / g.pack;
+  g.tile_tokens = kSvRows / g.pack;
+}
+
+// A tile's queries: tile_tokens tokens x pack heads x 64 columns.
+bool map_queries(CUtensorMap* m, const ServingArgs& g, uint32_t dtype, const int64_t (&q_stride)[2]) {
+  return map_heads(m, g.q, dtype, 3,
+                   {static_cast<uint64_t>(g.head_dim), static_cast<uint64_t>(g.q_heads),
+                    static_cast<uint64_t>(g.total_q), 1},
+                   {q_stride[1], q_stride[0], 0},
+                   {static_cast<uint32_t>(g.pack), static_cast<uint32_t>(g.tile_tokens), 1});
+}
+
 template <int DP, typename T>
-int launch_prompt(const CUtensorMap& tk, const CUtensorMap& tv, const ServingArgs& g, int blocks, cudaStream_t st) {
+int launch_prompt(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const ServingArgs& g, int blocks,
+                  cudaStream_t st) {
   auto kern = serving_attention_kernel<DP, T, false, true>;
   constexpr int smem = SvSmem<DP, true>::kBytes;
   static SmemGrant grant;
   if (const int rc = grant(reinterpret_cast<const void*>(kern), smem)) return rc;
-  kern<<<blocks, kSvThreads, smem, st>>>(tk, tv, g);
+  kern<<<blocks, kSvThreads, smem, st>>>(tq, tk, tv, g);
   return launch_status();
 }
 
 // The attention over a cache with items of kTileRows rows, then the join of
 // its cut items.
 template <int DP, typename T, int kTileRows>
-int launch_cache(const CUtensorMap& tk, const CUtensorMap& tv, const ServingArgs& g, int blocks, cudaStream_t st) {
+int launch_cache(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const ServingArgs& g, int blocks,
+                 cudaStream_t st) {
   static SmemGrant grant;
   int rc;
   if constexpr (kTileRows >= kSvRows) {
@@ -312,7 +331,7 @@ int launch_cache(const CUtensorMap& tk, const CUtensorMap& tv, const ServingArgs
     auto kern = serving_attention_kernel<DP, T, true, kPair>;
     constexpr int smem = SvSmem<DP, kPair>::kBytes;
     if ((rc = grant(reinterpret_cast<const void*>(kern), smem))) return rc;
-    kern<<<blocks, kSvThreads, smem, st>>>(tk, tv, g);
+    kern<<<blocks, kSvThreads, smem, st>>>(tq, tk, tv, g);
   } else {
     auto kern = decode_attention_kernel<DP, T, kTileRows>;
     constexpr int smem = DcSmem<DP, kTileRows>::kBytes;
@@ -339,14 +358,14 @@ int launch_cache(const CUtensorMap& tk, const CUtensorMap& tv, const ServingArgs
 }
 
 template <int DP, typename T>
-int launch_cache_rows(int rows, const CUtensorMap& tk, const CUtensorMap& tv, const ServingArgs& g, int blocks,
-                      cudaStream_t st) {
+int launch_cache_rows(int rows, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                      const ServingArgs& g, int blocks, cudaStream_t st) {
   switch (rows) {
-    case 16: return launch_cache<DP, T, 16>(tk, tv, g, blocks, st);
-    case 32: return launch_cache<DP, T, 32>(tk, tv, g, blocks, st);
-    case 64: return launch_cache<DP, T, 64>(tk, tv, g, blocks, st);
-    case 128: return launch_cache<DP, T, 128>(tk, tv, g, blocks, st);
-    default: return launch_cache<DP, T, 256>(tk, tv, g, blocks, st);
+    case 16: return launch_cache<DP, T, 16>(tq, tk, tv, g, blocks, st);
+    case 32: return launch_cache<DP, T, 32>(tq, tk, tv, g, blocks, st);
+    case 64: return launch_cache<DP, T, 64>(tq, tk, tv, g, blocks, st);
+    case 128: return launch_cache<DP, T, 128>(tq, tk, tv, g, blocks, st);
+    default: return launch_cache<DP, T, 256>(tq, tk, tv, g, blocks, st);
   }
 }
 
@@ -368,8 +387,7 @@ int run_prompt_attention(const akili_prompt_attention_arg_t* a, cudaStream_t st)
   DevInfo di;
   if ((rc = device_info(&di))) return rc;
   const uint64_t group = a->q_heads / a->kv_heads;
-  const uint64_t blocks = ((a->total_q * group + 2 * kSvRows - 1) / (2 * kSvRows) + a->batch) * a->kv_heads;
-  if (a->total_q * group > (1u << 30) || blocks > INT32_MAX) return AKILI_E_SHAPE;
+  if (a->total_q * group > (1u << 30)) return AKILI_E_SHAPE;
   ServingArgs g{};
   g.q = P(a->q_addr); g.o = W(a->o_addr);
   g.lse = static_cast<float*>(W(a->lse_addr));
@@ -378,25 +396,31 @@ int run_prompt_attention(const akili_prompt_attention_arg_t* a, cudaStream_t st)
   g.q_heads = a->q_heads; g.kv_heads = a->kv_heads; g.group = static_cast<int>(group);
   g.head_dim = a->head_dim; g.batch = a->batch;
   g.total_q = a->total_q; g.total_k = a->total_k; g.causal = a->causal;
+  pack_heads(g);
+  // at most one tile pair of a sequence is not full
+  const uint64_t blocks =
+      (a->total_q / (2 * static_cast<uint64_t>(g.tile_tokens)) + a->batch) * g.head_groups;
+  if (blocks > INT32_MAX) return AKILI_E_SHAPE;
   g.scale_log2 = scale_log2_of(a->softmax_scale, a->head_dim);
   for (int i = 0; i < 2; ++i) { g.q_st[i] = a->q_stride[i]; g.o_st[i] = a->o_stride[i]; }
   const uint64_t per_head = static_cast<uint64_t>(a->total_k) * a->head_dim * 4;  // bytes of K and V
-  g.chunk_heads = static_cast<int>(
-      std::min<uint64_t>(std::max<uint64_t>(kPromptChunkBytes / std::max<uint64_t>(per_head, 1), 1), a->kv_heads));
+  g.chunk_heads = static_cast<int>(std::min<uint64_t>(
+      std::max<uint64_t>(kPromptChunkBytes / std::max<uint64_t>(per_head, 1), 1) * g.groups_per_kv, g.head_groups));
   // without any key the maps are never used; they are made over q then
   const bool keys = a->total_k > 0;
   const uint64_t dim[4] = {a->head_dim, keys ? a->kv_heads : 1, keys ? a->total_k : 1, 1};
-  CUtensorMap tk, tv;
-  if (!map_heads(&tk, P(keys ? a->k_addr : a->q_addr), a->dtype, 3, dim, {a->k_stride[1], a->k_stride[0], 0}, 2,
-                 kSvKeys) ||
-      !map_heads(&tv, P(keys ? a->v_addr : a->q_addr), a->dtype, 3, dim, {a->v_stride[1], a->v_stride[0], 0}, 2,
-                 kSvKeys))
+  CUtensorMap tq, tk, tv;
+  if (!map_heads(&tk, P(keys ? a->k_addr : a->q_addr), a->dtype, 3, dim, {a->k_stride[1], a->k_stride[0], 0},
+                 {1, kSvKeys, 1}) ||
+      !map_heads(&tv, P(keys ? a->v_addr : a->q_addr), a->dtype, 3, dim, {a->v_stride[1], a->v_stride[0], 0},
+                 {1, kSvKeys, 1}) ||
+      !map_queries(&tq, g, a->dtype, a->q_stride))
     return AKILI_E_LAUNCH;
   const int n = static_cast<int>(blocks);
   if (a->dtype == AKILI_DTYPE_BF16)
-    return g.head_dim <= 64 ? launch_prompt<64, __nv_bfloat16>(tk, tv, g, n, st)
-                            : launch_prompt<128, __nv_bfloat16>(tk, tv, g, n, st);
-  return g.head_dim <= 64 ? launch_prompt<64, __half>(tk, tv, g, n, st) : launch_prompt<128, __half>(tk, tv, g, n, st);
+    return g.head_dim <= 64 ? launch_prompt<64, __nv_bfloat16>(tq, tk, tv, g, n, st)
+                            : launch_prompt<128, __nv_bfloat16>(tq, tk, tv, g, n, st);
+  return g.head_dim <= 64 ? launch_prompt<64, __half>(tq, tk, tv, g, n, st) : launch_prompt<128, __half>(tq, tk, tv, g, n, st);
 }
 
 int check_tree(const akili_tree_attention_arg_t* a) {
@@ -464,19 +488,28 @@ int run_tree_attention(const akili_tree_attention_arg_t* a, cudaStream_t st) {
   for (int i = 0; i < 2; ++i) { g.q_st[i] = a->q_stride[i]; g.o_st[i] = a->o_stride[i]; }
   g.table_stride = a->page_table_stride;
   g.mask_stride = a->mask_stride;
-  const uint64_t dim[4] = {a->head_dim, a->page_size, a->kv_heads, a->num_pages};
-  CUtensorMap tk, tv;
-  if (!map_heads(&tk, P(a->k_pages_addr), a->dtype, 4, dim,
-                 {a->k_page_stride[1], a->k_page_stride[2], a->k_page_stride[0]}, 1, g.box_rows) ||
-      !map_heads(&tv, P(a->v_pages_addr), a->dtype, 4, dim,
-                 {a->v_page_stride[1], a->v_page_stride[2], a->v_page_stride[0]}, 1, g.box_rows))
-    return AKILI_E_LAUNCH;
   const int rows = tree_tile_rows(a);
+  if (rows >= kSvRows) {
+    pack_heads(g);
+  } else {  // the few-row form takes a group's heads whole
+    g.pack = g.group;
+    g.head_groups = g.kv_heads;
+    g.groups_per_kv = 1;
+    g.tile_tokens = 1;
+  }
+  const uint64_t dim[4] = {a->head_dim, a->page_size, a->kv_heads, a->num_pages};
+  CUtensorMap tq = {}, tk, tv;
+  if (!map_heads(&tk, P(a->k_pages_addr), a->dtype, 4, dim,
+                 {a->k_page_stride[1], a->k_page_stride[2], a->k_page_stride[0]}, {static_cast<uint32_t>(g.box_rows), 1, 1}) ||
+      !map_heads(&tv, P(a->v_pages_addr), a->dtype, 4, dim,
+                 {a->v_page_stride[1], a->v_page_stride[2], a->v_page_stride[0]}, {static_cast<uint32_t>(g.box_rows), 1, 1}) ||
+      (rows >= kSvRows && !map_queries(&tq, g, a->dtype, a->q_stride)))
+    return AKILI_E_LAUNCH;
   if (a->dtype == AKILI_DTYPE_BF16)
-    return g.head_dim <= 64 ? launch_cache_rows<64, __nv_bfloat16>(rows, tk, tv, g, di.sms, st)
-                            : launch_cache_rows<128, __nv_bfloat16>(rows, tk, tv, g, di.sms, st);
-  return g.head_dim <= 64 ? launch_cache_rows<64, __half>(rows, tk, tv, g, di.sms, st)
-                          : launch_cache_rows<128, __half>(rows, tk, tv, g, di.sms, st);
+    return g.head_dim <= 64 ? launch_cache_rows<64, __nv_bfloat16>(rows, tq, tk, tv, g, di.sms, st)
+                            : launch_cache_rows<128, __nv_bfloat16>(rows, tq, tk, tv, g, di.sms, st);
+  return g.head_dim <= 64 ? launch_cache_rows<64, __half>(rows, tq, tk, tv, g, di.sms, st)
+                          : launch_cache_rows<128, __half>(rows, tq, tk, tv, g, di.sms, st);
 }
 
 }  // namespace
