@@ -62,7 +62,11 @@ constexpr int kSvRows = 128;  // rows of a tile
 constexpr int kSvKeys = 128;  // keys of a block
 constexpr int kSvThreads = 640;
 constexpr int kSvJoinThreads = 256;
-constexpr int kSvJoinSplit = 4;  // blocks that share the rows of a cut item
+// Blocks that share a cut item: the rows of the few-row form, the columns of
+// the row forms (256 rows x 128 columns: 8 blocks 88 -> XX us a drafted batch
+// against 4).
+template <int kTileRows>
+constexpr int kSvJoinSplit = kTileRows < kSvRows ? (kTileRows + 7) / 8 : kTileRows / 32;
 
 struct ServingArgs {
   const void* q;
@@ -251,13 +255,13 @@ __device__ __forceinline__ int sv_levels(const ServingArgs& a, int b) {
   return (n + 2 * a.tile_tokens - 1) / (2 * a.tile_tokens);
 }
 struct SvPromptLine {
-  int mine;         // levels of sequence `lane`
-  int top;          // most levels of any sequence
-  long long tiles;  // tile pairs of a head group
-  __device__ __forceinline__ long long at_least(const ServingArgs& a, int l) const {  // tile pairs of level l and above
-    long long c = max(mine - l, 0);
+  int mine;   // levels of sequence `lane`
+  int top;    // most levels of any sequence
+  int tiles;  // tile pairs of a head group
+  __device__ __forceinline__ int at_least(const ServingArgs& a, int l) const {  // tile pairs of level l and above
+    int c = max(mine - l, 0);
     for (int b0 = 32; b0 < a.batch; b0 += 32) c += max(sv_levels(a, b0 + static_cast<int>(lane_id())) - l, 0);
-    return warp_sum(c);
+    return __reduce_add_sync(0xffffffffu, c);
   }
   __device__ __forceinline__ void load(const ServingArgs& a) {
     mine = sv_levels(a, static_cast<int>(lane_id()));
@@ -266,13 +270,15 @@ struct SvPromptLine {
     top = __reduce_max_sync(0xffffffffu, top);
     tiles = at_least(a, 0);
   }
-  __device__ __forceinline__ bool find(const ServingArgs& a, long long id, int* b_out, int* hk, int* level) const {
-    if (id >= tiles * a.head_groups) return false;
-    const long long chunk = id / (tiles * a.chunk_heads);
-    const long long rem = id - chunk * tiles * a.chunk_heads;
-    const int heads = min(a.chunk_heads, a.head_groups - static_cast<int>(chunk) * a.chunk_heads);
-    const long long x = rem / heads;
-    *hk = static_cast<int>(chunk) * a.chunk_heads + static_cast<int>(rem - x * heads);
+  // (the grid has fewer than 2^31 blocks, so 32 bits hold every count)
+  __device__ __forceinline__ bool find(const ServingArgs& a, uint32_t id, int* b_out, int* hk, int* level) const {
+    const uint32_t all = static_cast<uint32_t>(tiles);
+    if (tiles == 0 || id / all >= static_cast<uint32_t>(a.head_groups)) return false;
+    const uint32_t per = all * static_cast<uint32_t>(a.chunk_heads);  // of a chunk
+    const uint32_t chunk = id / per, rem = id - chunk * per;
+    const uint32_t heads = min(a.chunk_heads, a.head_groups - static_cast<int>(chunk) * a.chunk_heads);
+    const int x = static_cast<int>(rem / heads);
+    *hk = static_cast<int>(chunk) * a.chunk_heads + static_cast<int>(rem - static_cast<uint32_t>(x) * heads);
     int lo = 0, hi = top - 1;  // the last level with more than x tile pairs at or above it
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -280,13 +286,13 @@ struct SvPromptLine {
       else hi = mid - 1;
     }
     *level = lo;
-    long long left = x - at_least(a, lo + 1);
+    int left = x - at_least(a, lo + 1);
     for (int b0 = 0; b0 < a.batch; b0 += 32) {
       const int levels = b0 == 0 ? mine : sv_levels(a, b0 + static_cast<int>(lane_id()));
       const unsigned on = __ballot_sync(0xffffffffu, levels > lo);
       const int c = __popc(on);
       if (left < c) {
-        *b_out = b0 + __fns(on, 0, static_cast<int>(left) + 1);
+        *b_out = b0 + __fns(on, 0, left + 1);
         return true;
       }
       left -= c;
@@ -488,6 +494,18 @@ __global__ void __maxnreg__(96)
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
+  // the scheduler finds its place meanwhile
+  SvPromptLine line;
+  SvWalk<kTileRows> walk;
+  bool more = true;
+  if (warp == 19) {
+    if constexpr (kPaged) {
+      long long quota, total;
+      more = sv_share<kTileRows>(a, blockIdx.x, gridDim.x, walk, &quota, &total);
+    } else {
+      line.load(a);
+    }
+  }
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ctl->tmem;
@@ -514,15 +532,6 @@ __global__ void __maxnreg__(96)
     uint32_t count = 0;            // pieces handed out
     uint32_t q_used[2] = {0, 0};   // loads of each Q tile
     uint32_t asked = 0;            // requests for further blocks
-    SvPromptLine line;
-    SvWalk<kTileRows> walk;
-    bool more = ok;
-    if constexpr (kPaged) {
-      long long quota, total;
-      if (ok) more = sv_share<kTileRows>(a, blockIdx.x, gridDim.x, walk, &quota, &total);
-    } else {
-      line.load(a);
-    }
     uint32_t id = blockIdx.x;
     while (ok) {
       SvPiece p;
@@ -1157,38 +1166,48 @@ __global__ void __launch_bounds__(kSvJoinThreads) attention_join_kernel(const __
       return t < a.tile_tokens && *tok < tokens;
     }
   };
-  constexpr int kUnits = kByRow ? 32 : DP / 4;  // threads of a row
-  const int step = gridDim.y * kSvJoinThreads;
-  for (int x = blockIdx.y * kSvJoinThreads + threadIdx.x; x < kTileRows * kUnits; x += step) {
-    const int r = kByRow ? x / kUnits : x % kTileRows, unit = kByRow ? x % kUnits : x / kTileRows;
+  auto join_row = [&](int r, int unit0, int unit_step) {
     int tok, head;
-    if (!row_of(r, &tok, &head) || unit * 4 >= a.head_dim) continue;
+    if (!row_of(r, &tok, &head)) return;
     float m = -INFINITY;
+#pragma unroll 4
     for (int i = 0; i < parts; ++i) m = fmaxf(m, part(i)[kM + r]);
     const float m_sub = m == -INFINITY ? 0.0f : m;
-    float o[4] = {}, l = 0.0f;
+    float l = 0.0f;
 #pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-      const float* p = part(i);
-      const float w = exp2f(p[kM + r] - m_sub);
-      l += w * p[kL + r];
-      if (w != 0.0f) {
-        const float4 v = *reinterpret_cast<const float4*>(
-            p + (kByRow ? static_cast<size_t>(r) * DP + unit * 4 : (static_cast<size_t>(unit) * kTileRows + r) * 4));
-        o[0] += w * v.x;
-        o[1] += w * v.y;
-        o[2] += w * v.z;
-        o[3] += w * v.w;
-      }
-    }
+    for (int i = 0; i < parts; ++i) l += exp2f(part(i)[kM + r] - m_sub) * part(i)[kL + r];
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
     const long long qrow = q0 + tok;
     const int qh = hk * (kByRow ? a.group : a.pack) + head;
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-    uint2 v;
-    v.x = pack2<T>(o[0] * inv, o[1] * inv);
-    v.y = pack2<T>(o[2] * inv, o[3] * inv);
-    *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + qrow * a.o_st[0] + qh * a.o_st[1] + unit * 4) = v;
-    if (a.lse != nullptr && unit == 0) a.lse[qrow * a.q_heads + qh] = (m + log2f(l)) * 0.6931471805599453f;
+#pragma unroll 2
+    for (int unit = unit0; unit * 4 < a.head_dim; unit += unit_step) {
+      float o[4] = {};
+#pragma unroll 4
+      for (int i = 0; i < parts; ++i) {
+        const float* p = part(i);
+        const float w = exp2f(p[kM + r] - m_sub);
+        const float4 v = *reinterpret_cast<const float4*>(
+            p + (kByRow ? static_cast<size_t>(r) * DP + unit * 4 : (static_cast<size_t>(unit) * kTileRows + r) * 4));
+        if (w != 0.0f) {  // (a part that saw nothing of the row holds anything)
+          o[0] += w * v.x;
+          o[1] += w * v.y;
+          o[2] += w * v.z;
+          o[3] += w * v.w;
+        }
+      }
+      uint2 v;
+      v.x = pack2<T>(o[0] * inv, o[1] * inv);
+      v.y = pack2<T>(o[2] * inv, o[3] * inv);
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + qrow * a.o_st[0] + qh * a.o_st[1] + unit * 4) = v;
+    }
+    if (a.lse != nullptr && unit0 == 0) a.lse[qrow * a.q_heads + qh] = (m + log2f(l)) * 0.6931471805599453f;
+  };
+  if constexpr (kByRow) {
+    for (int r = blockIdx.y * (kSvJoinThreads / 32) + warp; r < kTileRows; r += gridDim.y * (kSvJoinThreads / 32))
+      join_row(r, lane, 32);
+  } else {
+    constexpr int kPer = kSvJoinThreads / kTileRows;  // threads of a row within a block
+    join_row(threadIdx.x % kTileRows, blockIdx.y * kPer + threadIdx.x / kTileRows, gridDim.y * kPer);
   }
 }
 

@@ -345,7 +345,7 @@ int launch_cache(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(blocks, kSvJoinSplit);
+  cfg.gridDim = dim3(blocks, kSvJoinSplit<kTileRows>);
   cfg.blockDim = dim3(kSvJoinThreads);
   cfg.stream = st;
   cfg.attrs = &attr;
