@@ -53,10 +53,7 @@ struct DcControl {
   uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], pv_done[2], o_full[2], o_empty[2];
   uint64_t drain;
   uint32_t tmem;
-  int work;
-  int b;
   volatile int abort[2];  // a wait that gave up before the barrier of this parity
-  long long begin, end, off;
 };
 
 // Reduces v[n] over the warp's lanes by halving: after it lane L holds the
@@ -137,20 +134,7 @@ __global__ void __launch_bounds__(kDcThreads, 1)
   const uint32_t lane = lane_id();
   griddep_launch_dependents();
 
-  if (warp == 0) {
-    SvWalk<N> w;
-    long long quota, total;
-    const bool work = sv_share<N>(a, blockIdx.x, gridDim.x, w, &quota, &total);
-    if (lane == 0) {
-      ctl->work = work && (smem_u32(smem) & 1023) == 0;
-      if (work) {
-        ctl->b = w.b;
-        ctl->begin = w.begin;
-        ctl->end = w.end;
-        ctl->off = w.off;
-      }
-    }
-  } else if (warp == 1) {
+  if (warp == 3) {
     if (lane == 0) {
       tma_prefetch_desc(&tmK);
       tma_prefetch_desc(&tmV);
@@ -175,25 +159,30 @@ __global__ void __launch_bounds__(kDcThreads, 1)
       mbar_init(&ctl->drain, 1);
       fence_mbar_init();
     }
+    __syncwarp();
   } else if (warp == 2) {
     tmem_alloc(&ctl->tmem, kTmemCols);
     tmem_relinquish();
   }
+  // Every warp finds the CTA's share by itself and the loaders look up their
+  // first pages before the barrier: the first load leaves that much earlier
+  // (5500 -> XXXX cycles after the start).
+  SvWalk<N> walk;
+  SvPiece pc;
+  long long quota, total;
+  const bool work = sv_share<N>(a, blockIdx.x, gridDim.x, walk, &quota, &total) && (smem_u32(smem) & 1023) == 0;
+  auto next = [&]() { return work && walk.next(a, blockIdx.x, pc); };
+  // lane b looks up the page of box b (box_rows keys) of block j of the piece
+  auto lookup = [&](int j) -> int {
+    const int in = static_cast<int>(lane) * a.box_rows;
+    const int key = (pc.kb + j) * kSvKeys + in;
+    return j < pc.loads && in < kSvKeys && key < pc.s.m ? a.page_table[pc.b * a.table_stride + key / a.page_size] : 0;
+  };
+  bool have = next();
+  int page = have && warp < 2 ? lookup(0) : 0;
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ctl->tmem;
-  const bool work = ctl->work != 0;
-  SvWalk<N> walk;
-  if (work) {
-    walk.begin = walk.pos = ctl->begin;
-    walk.end = ctl->end;
-    walk.off = ctl->off;
-    walk.b = ctl->b;
-    bool clamped;
-    walk.load(a, &clamped);
-  }
-  SvPiece pc;
-  auto next = [&]() { return work && walk.next(a, blockIdx.x, pc); };
 
   if (warp < 2) {
     // ------------------------------------------------------ key / value loads
@@ -206,28 +195,18 @@ __global__ void __launch_bounds__(kDcThreads, 1)
     int st = 0;
     uint32_t round = 0, issued = 0;
     bool ok = true;
-    while (ok && next()) {
-      const int* table = a.page_table + pc.b * a.table_stride;
-      // lane b looks up the page of box b (box_rows keys), a block ahead
-      auto lookup = [&](int j) -> int {
-        const int key = (pc.kb + j) * kSvKeys + static_cast<int>(lane) * a.box_rows;
-        int page = 0;
-        if (j < pc.loads && static_cast<int>(lane) * a.box_rows < kSvKeys && key < pc.s.m) {
-          page = table[key / a.page_size];
-          if (page < 0 || page >= a.num_pages) {  // outside the tensor: TMA fills zeros
-            record_bad_index();
-            page = -1;
-          }
-        }
-        return page;
-      };
-      int page = lookup(0);
+    for (bool first = true; ok && have; have = next(), first = false) {
+      if (!first) page = lookup(0);
+      int ahead = lookup(1);
       for (int j = 0; j < pc.loads; ++j) {
         const int key0 = (pc.kb + j) * kSvKeys;
         const int boxes = (min(kSvKeys, pc.s.m - key0) + a.box_rows - 1) / a.box_rows;
-        const int ahead = lookup(j + 1);
         if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], (round - 1) & 1, kSiteFlashFree));
         if (!ok) break;
+        if (page < 0 || page >= a.num_pages) {  // outside the tensor: TMA fills zeros
+          record_bad_index();
+          page = -1;
+        }
         if (lane == 0) mbar_expect_tx(&full[st], static_cast<uint32_t>(boxes * a.box_rows * 128 * kChunks));
         __syncwarp();
         const uint32_t dst = smem_u32(ring + st * L::kKV), bar = smem_u32(&full[st]);
@@ -243,6 +222,7 @@ __global__ void __launch_bounds__(kDcThreads, 1)
         }
         ++issued;
         page = ahead;
+        ahead = lookup(j + 2);
         if (++st == stages) {
           st = 0;
           ++round;
@@ -306,8 +286,15 @@ __global__ void __launch_bounds__(kDcThreads, 1)
         ++vr;
       }
     };
-    while (ok && next()) {
+    for (; ok && have; have = next()) {
       for (int j = 0; j < pc.loads && ok; ++j) {
+        // The product of the block before goes first where its successor's keys
+        // are still on their way.
+        if (held && !__all_sync(0xffffffffu, mbar_try_wait(smem_u32(&ctl->k_full[ks]), kr & 1))) {
+          issue_pv();
+          held = false;
+          if (!ok) break;
+        }
         if (j == 0) wait(&ctl->q_full[item & 1], (item >> 1) & 1, kSiteFlashQ);
         wait(&ctl->k_full[ks], kr & 1, kSiteFlashKV);
         if (!ok) break;
@@ -345,7 +332,7 @@ __global__ void __launch_bounds__(kDcThreads, 1)
     // rows x 16-byte columns over the lanes, K-major with the 128-byte swizzle
     uint32_t item = 0;
     bool ok = true;
-    for (; ok && next(); ++item) {
+    for (; ok && have; ++item, have = next()) {
       if (item >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&ctl->q_empty[item & 1], ((item >> 1) - 1) & 1, kSiteFlashFree));
       if (!ok) break;
       uint8_t* dst = smem + L::kQOff + (item & 1) * L::kQ;
@@ -379,7 +366,7 @@ __global__ void __launch_bounds__(kDcThreads, 1)
     uint32_t g = 0, item = 0;
     bool alive = true;
     float m[N], l[N];
-    for (; alive && next(); ++item) {
+    for (; alive && have; ++item, have = next()) {
 #pragma unroll
       for (int n = 0; n < N; ++n) {
         m[n] = -3.4028235e38f;  // "nothing seen": any finite score passes it

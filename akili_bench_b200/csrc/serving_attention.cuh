@@ -63,8 +63,7 @@ constexpr int kSvKeys = 128;  // keys of a block
 constexpr int kSvThreads = 640;
 constexpr int kSvJoinThreads = 256;
 // Blocks that share a cut item: the rows of the few-row form, the columns of
-// the row forms (256 rows x 128 columns: 8 blocks 88 -> XX us a drafted batch
-// against 4).
+// the row forms.
 template <int kTileRows>
 constexpr int kSvJoinSplit = kTileRows < kSvRows ? (kTileRows + 7) / 8 : kTileRows / 32;
 
@@ -199,15 +198,15 @@ __device__ __forceinline__ long long warp_scan(long long v) {  // inclusive
 }
 
 // Blocks of sequence b on the line (0 past the batch).
+// Sequence b's place on the line (no blocks past the batch).
 template <int kTileRows>
-__device__ __forceinline__ long long sv_line_blocks(const ServingArgs& a, int b, bool record) {
-  if (b >= a.batch) return 0;
-  SvWalk<kTileRows> w;
+__device__ __forceinline__ void sv_line_sequence(const ServingArgs& a, int b, bool record, SvWalk<kTileRows>& w) {
   w.b = b;
+  w.size = 0;
+  if (b >= a.batch) return;
   bool clamped;
   w.load(a, &clamped);
   if (record && clamped) record_bad_index();
-  return w.size;
 }
 
 // The share of CTA `cta` of `ctas` (one warp): false if it is empty.
@@ -215,11 +214,19 @@ template <int kTileRows>
 __device__ __forceinline__ bool sv_share(const ServingArgs& a, int cta, int ctas, SvWalk<kTileRows>& w,
                                          long long* quota_out, long long* total_out) {
   const int lane = threadIdx.x & 31;
-  const long long first = sv_line_blocks<kTileRows>(a, lane, cta == 0);
-  long long total = first;
-  for (int b0 = 32; b0 < a.batch; b0 += 32) total += sv_line_blocks<kTileRows>(a, b0 + lane, cta == 0);
+  SvWalk<kTileRows> mine;
+  sv_line_sequence<kTileRows>(a, lane, cta == 0, mine);
+  long long total = mine.size;
+  for (int b0 = 32; b0 < a.batch; b0 += 32) {
+    SvWalk<kTileRows> more;
+    sv_line_sequence<kTileRows>(a, b0 + lane, cta == 0, more);
+    total += more.size;
+  }
   total = warp_sum(total);
-  const long long quota = (total + ctas - 1) / ctas;
+  // (a 64-bit division costs some 100 cycles more)
+  const long long quota = total + ctas <= 0xffffffffll
+                              ? static_cast<uint32_t>(total + ctas - 1) / static_cast<uint32_t>(ctas)
+                              : (total + ctas - 1) / ctas;
   *quota_out = quota;
   *total_out = total;
   w.begin = w.pos = cta * quota;
@@ -227,15 +234,21 @@ __device__ __forceinline__ bool sv_share(const ServingArgs& a, int cta, int ctas
   if (w.begin >= total) return false;
   long long before = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
-    const long long mine = b0 == 0 ? first : sv_line_blocks<kTileRows>(a, b0 + lane, false);
-    const long long upto = before + warp_scan(mine);
+    if (b0 > 0) sv_line_sequence<kTileRows>(a, b0 + lane, false, mine);
+    const long long upto = before + warp_scan(mine.size);
     const unsigned hit = __ballot_sync(0xffffffffu, upto > w.begin);
     if (hit) {
       const int at = __ffs(hit) - 1;
       w.b = b0 + at;
-      w.off = w.begin - __shfl_sync(0xffffffffu, upto - mine, at);
-      bool clamped;
-      w.load(a, &clamped);
+      w.off = w.begin - __shfl_sync(0xffffffffu, upto - mine.size, at);
+      w.size = __shfl_sync(0xffffffffu, mine.size, at);
+      w.tiles = __shfl_sync(0xffffffffu, mine.tiles, at);
+      w.blocks = __shfl_sync(0xffffffffu, mine.blocks, at);
+      w.s.q0 = __shfl_sync(0xffffffffu, mine.s.q0, at);
+      w.s.n = __shfl_sync(0xffffffffu, mine.s.n, at);
+      w.s.k0 = 0;
+      w.s.m = __shfl_sync(0xffffffffu, mine.s.m, at);
+      w.s.sure = __shfl_sync(0xffffffffu, mine.s.sure, at);
       return true;
     }
     before = __shfl_sync(0xffffffffu, upto, 31);
@@ -654,25 +667,22 @@ __global__ void __maxnreg__(96)
         if constexpr (kPaged) {
           const int in = static_cast<int>(lane) * a.box_rows;
           const int key = (kb + j) * kSvKeys + in;
-          if (j < loads && in < kSvKeys && key < m) {
-            page = table[key / a.page_size];
-            if (page < 0 || page >= a.num_pages) {  // outside the tensor: TMA fills zeros
-              record_bad_index();
-              page = -1;
-            }
-          }
+          if (j < loads && in < kSvKeys && key < m) page = table[key / a.page_size];
         }
         return page;
       };
-      int page = lookup(0);
+      int page = lookup(0), ahead = lookup(1);
       for (int j = 0; j < loads; ++j) {
         const int key0 = (kb + j) * kSvKeys;
-        const int ahead = lookup(j + 1);
         if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], (round - 1) & 1, kSiteFlashFree));
         if (!ok) break;
         const uint32_t dst = smem_u32(ring + st * L::kKV), bar = smem_u32(&full[st]);
         if constexpr (kPaged) {
           const int boxes = (min(kSvKeys, m - key0) + a.box_rows - 1) / a.box_rows;
+          if (page < 0 || page >= a.num_pages) {  // outside the tensor: TMA fills zeros
+            record_bad_index();
+            page = -1;
+          }
           if (lane == 0) mbar_expect_tx(&full[st], static_cast<uint32_t>(boxes * a.box_rows * 128 * kChunks));
           __syncwarp();
           int in_page = key0 % a.page_size;
@@ -693,6 +703,7 @@ __global__ void __maxnreg__(96)
         }
         ++issued;
         page = ahead;
+        ahead = lookup(j + 2);
         if (++st == kStages) {
           st = 0;
           ++round;
@@ -1166,41 +1177,54 @@ __global__ void __launch_bounds__(kSvJoinThreads) attention_join_kernel(const __
       return t < a.tile_tokens && *tok < tokens;
     }
   };
+  // Eight parts at a time, all of whose loads are under way together.
   auto join_row = [&](int r, int unit0, int unit_step) {
     int tok, head;
     if (!row_of(r, &tok, &head)) return;
-    float m = -INFINITY;
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) m = fmaxf(m, part(i)[kM + r]);
-    const float m_sub = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f;
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) l += exp2f(part(i)[kM + r] - m_sub) * part(i)[kL + r];
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
     const long long qrow = q0 + tok;
     const int qh = hk * (kByRow ? a.group : a.pack) + head;
-#pragma unroll 2
     for (int unit = unit0; unit * 4 < a.head_dim; unit += unit_step) {
-      float o[4] = {};
-#pragma unroll 4
-      for (int i = 0; i < parts; ++i) {
-        const float* p = part(i);
-        const float w = exp2f(p[kM + r] - m_sub);
-        const float4 v = *reinterpret_cast<const float4*>(
-            p + (kByRow ? static_cast<size_t>(r) * DP + unit * 4 : (static_cast<size_t>(unit) * kTileRows + r) * 4));
-        if (w != 0.0f) {  // (a part that saw nothing of the row holds anything)
-          o[0] += w * v.x;
-          o[1] += w * v.y;
-          o[2] += w * v.z;
-          o[3] += w * v.w;
+      float o[4] = {}, m = -INFINITY, l = 0.0f;
+      for (int i0 = 0; i0 < parts; i0 += 8) {
+        float pm[8], pl[8];
+        float4 pv[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const bool on = i0 + i < parts;
+          const float* p = part(on ? i0 + i : i0);
+          pm[i] = on ? p[kM + r] : -INFINITY;
+          pl[i] = p[kL + r];
+          pv[i] = *reinterpret_cast<const float4*>(
+              p + (kByRow ? static_cast<size_t>(r) * DP + unit * 4 : (static_cast<size_t>(unit) * kTileRows + r) * 4));
+        }
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, pm[i]);
+        const float sub = top == -INFINITY ? 0.0f : top;
+        const float keep = exp2f(m - sub);
+        m = top;
+        l *= keep;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[x] *= keep;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float w = exp2f(pm[i] - sub);
+          if (w != 0.0f) {  // (a part that saw nothing of the row holds anything)
+            l += w * pl[i];
+            o[0] += w * pv[i].x;
+            o[1] += w * pv[i].y;
+            o[2] += w * pv[i].z;
+            o[3] += w * pv[i].w;
+          }
         }
       }
+      const float inv = l != 0.0f ? 1.0f / l : 0.0f;
       uint2 v;
       v.x = pack2<T>(o[0] * inv, o[1] * inv);
       v.y = pack2<T>(o[2] * inv, o[3] * inv);
       *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + qrow * a.o_st[0] + qh * a.o_st[1] + unit * 4) = v;
+      if (a.lse != nullptr && unit == 0) a.lse[qrow * a.q_heads + qh] = (m + log2f(l)) * 0.6931471805599453f;
     }
-    if (a.lse != nullptr && unit0 == 0) a.lse[qrow * a.q_heads + qh] = (m + log2f(l)) * 0.6931471805599453f;
   };
   if constexpr (kByRow) {
     for (int r = blockIdx.y * (kSvJoinThreads / 32) + warp; r < kTileRows; r += gridDim.y * (kSvJoinThreads / 32))
