@@ -24,6 +24,8 @@ __device__ __forceinline__ int find_sequence(const int* cu, int batch, int t) {
 // child, so the walk ends; one that is not ends it and is recorded.
 __global__ void __launch_bounds__(128) tree_mask_kernel(const int* parents, const int* cu_q, unsigned int* mask,
                                                         int batch, int total, int words) {
+  griddep_wait();
+  griddep_launch_dependents();
   const int t = blockIdx.x * 128 + threadIdx.x;
   if (t >= total) return;
   unsigned int* row = mask + static_cast<long long>(t) * words;
@@ -68,6 +70,8 @@ constexpr int kAcceptRows = 128;  // moves whose offsets are held at a time
 // come before its stores.
 template <typename U>
 __global__ void __launch_bounds__(kAcceptThreads) cache_accept_kernel(const AcceptArgs a) {
+  griddep_wait();
+  griddep_launch_dependents();
   const int layer = blockIdx.z;
   const int b = blockIdx.y;
   const int ctx = a.context_lens[b];

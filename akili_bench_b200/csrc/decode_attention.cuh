@@ -132,7 +132,6 @@ __global__ void __launch_bounds__(kDcThreads, 1)
   float* xchg = reinterpret_cast<float*>(smem + L::kXOff);
   const uint32_t warp = warp_id();
   const uint32_t lane = lane_id();
-  griddep_launch_dependents();
 
   if (warp == 3) {
     if (lane == 0) {
@@ -164,6 +163,10 @@ __global__ void __launch_bounds__(kDcThreads, 1)
     tmem_alloc(&ctl->tmem, kTmemCols);
     tmem_relinquish();
   }
+  // Nothing of an earlier kernel is read before it is complete; the join
+  // kernel, whose blocks read the lengths as they start, may start after that.
+  griddep_wait();
+  griddep_launch_dependents();
   // Every warp finds the CTA's share by itself and the loaders look up their
   // first pages before the barrier: the first load leaves that much earlier
   // (5500 -> XXXX cycles after the start).

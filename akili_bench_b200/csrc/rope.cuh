@@ -64,6 +64,8 @@ struct RopeArgs {
 template <typename T, int VEC, bool kAppend>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
   using V = ValueVec<T, VEC>;
+  griddep_wait();
+  griddep_launch_dependents();
   const int t = blockIdx.x;
   const int p = a.positions[t];
   if (p < 0 || p >= a.max_positions) {
@@ -182,6 +184,8 @@ struct RopeTableArgs {
 // cos | sin of p f_i in fp64: an fp32 product p f_i would be wrong by 4e-3 at
 // p = 131072.  Built once per model; 64 pairs x 131072 positions.
 __global__ void __launch_bounds__(256) rope_table_kernel(const __grid_constant__ RopeTableArgs a) {
+  griddep_wait();
+  griddep_launch_dependents();
   const int half = a.rot_dim / 2;
   const long long n = static_cast<long long>(a.max_positions) * half;
   for (long long e = blockIdx.x * 256ll + threadIdx.x; e < n; e += gridDim.x * 256ll) {

@@ -474,8 +474,6 @@ __global__ void __maxnreg__(96)
 
   const uint32_t warp = warp_id();
   const uint32_t lane = lane_id();
-  if constexpr (kPaged) griddep_launch_dependents();
-
   if (warp == 1) {
     tmem_alloc(&ctl->tmem, 512);
     tmem_relinquish();
@@ -507,6 +505,10 @@ __global__ void __maxnreg__(96)
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
+  // Nothing of an earlier kernel is read before it is complete; the join
+  // kernel, whose blocks read the lengths as they start, may start after that.
+  griddep_wait();
+  if constexpr (kPaged) griddep_launch_dependents();
   // the scheduler finds its place meanwhile
   SvPromptLine line;
   SvWalk<kTileRows> walk;
@@ -1159,6 +1161,7 @@ __global__ void __launch_bounds__(kSvJoinThreads) attention_join_kernel(const __
   }
   __syncthreads();
   griddep_wait();  // the parts
+  griddep_launch_dependents();
   if (parts == 0) return;
   constexpr size_t kSlot = static_cast<size_t>(kTileRows) * (DP + 2);
   auto part = [&](int i) { return a.parts + (i == 0 ? slot0 : 2 * (from + i)) * kSlot; };

@@ -29,6 +29,30 @@ bool all_multiples(const int64_t (&st)[n], int64_t of) {
   return true;
 }
 
+// The serving kernels are programmatic dependents of whatever runs before
+// them: a decode step is a chain of them, each a few microseconds long, and
+// one may be dispatched and set up while the one before drains.  Each waits
+// for its predecessor to complete before it touches memory.
+template <typename... Params, typename... Args>
+int launch_dependent(void (*kern)(Params...), dim3 grid, int threads, int smem, cudaStream_t st, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) {
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    cudaGetLastError();
+    return AKILI_E_LAUNCH;
+  }
+  return launch_status();
+}
+
 // ------------------------------------------------------------------- rope --
 template <typename T, int VEC, bool kAppend>
 int launch_rope(const DevInfo& di, const RopeArgs& r, cudaStream_t st) {
@@ -39,8 +63,7 @@ int launch_rope(const DevInfo& di, const RopeArgs& r, cudaStream_t st) {
   const int most = (heads + hl - 1) / hl;
   const int want = (4 * di.sms + r.tokens - 1) / r.tokens;
   const dim3 grid(r.tokens, std::min({most, want, 65535}));
-  rope_kernel<T, VEC, kAppend><<<grid, kRopeThreads, 0, st>>>(r);
-  return launch_status();
+  return launch_dependent(rope_kernel<T, VEC, kAppend>, grid, kRopeThreads, 0, st, r);
 }
 
 template <typename T, bool kAppend>
@@ -164,8 +187,8 @@ int run_rope_table(const akili_rope_table_arg_t* a, cudaStream_t st) {
   t.table = static_cast<float*>(W(a->table_addr));
   t.max_positions = a->max_positions;
   t.rot_dim = a->rot_dim;
-  rope_table_kernel<<<grid_for(di, static_cast<size_t>(a->max_positions) * half, 256, 8), 256, 0, st>>>(t);
-  return launch_status();
+  return launch_dependent(rope_table_kernel,
+                          dim3(grid_for(di, static_cast<size_t>(a->max_positions) * half, 256, 8)), 256, 0, st, t);
 }
 
 // ------------------------------------------------------------------ cache --
@@ -180,20 +203,18 @@ int run_tree_mask(const akili_tree_mask_arg_t* a, cudaStream_t st) {
   if ((rc = check_aligned({a->parents_addr, a->cu_q_addr, a->mask_addr}, 4))) return rc;
   DevInfo di;
   if ((rc = device_info(&di))) return rc;
-  tree_mask_kernel<<<(a->total_q + 127) / 128, 128, 0, st>>>(
-      static_cast<const int*>(P(a->parents_addr)), static_cast<const int*>(P(a->cu_q_addr)),
-      static_cast<unsigned int*>(W(a->mask_addr)), a->batch, a->total_q, a->mask_words);
-  return launch_status();
+  return launch_dependent(tree_mask_kernel, dim3((a->total_q + 127) / 128), 128, 0, st,
+                          static_cast<const int*>(P(a->parents_addr)), static_cast<const int*>(P(a->cu_q_addr)),
+                          static_cast<unsigned int*>(W(a->mask_addr)), static_cast<int>(a->batch),
+                          static_cast<int>(a->total_q), static_cast<int>(a->mask_words));
 }
 
 template <typename U>
-int launch_accept(const DevInfo& di, AcceptArgs g, const akili_cache_accept_arg_t* a, cudaStream_t st) {
+int launch_accept(AcceptArgs g, const akili_cache_accept_arg_t* a, cudaStream_t st) {
   g.vecs = static_cast<int>(a->head_dim * a->elem_bytes / sizeof(U));
   const int64_t cols = 2ll * a->kv_heads * g.vecs;
   const int share = static_cast<int>(std::min<int64_t>((cols + kAcceptThreads - 1) / kAcceptThreads, 1024));
-  cache_accept_kernel<U><<<dim3(share, a->batch, a->layers), kAcceptThreads, 0, st>>>(g);
-  (void)di;
-  return launch_status();
+  return launch_dependent(cache_accept_kernel<U>, dim3(share, a->batch, a->layers), kAcceptThreads, 0, st, g);
 }
 
 int run_cache_accept(const akili_cache_accept_arg_t* a, cudaStream_t st) {
@@ -233,10 +254,10 @@ int run_cache_accept(const akili_cache_accept_arg_t* a, cudaStream_t st) {
   g.table_stride = a->page_table_stride;
   g.acc_stride = a->accepted_stride;
   // 16-byte moves where every head row starts on 16 bytes, else element by element
-  if (bits % 16 == 0) return launch_accept<uint4>(di, g, a, st);
-  if (a->elem_bytes == 4) return launch_accept<uint32_t>(di, g, a, st);
-  if (a->elem_bytes == 2) return launch_accept<uint16_t>(di, g, a, st);
-  return launch_accept<uint8_t>(di, g, a, st);
+  if (bits % 16 == 0) return launch_accept<uint4>(g, a, st);
+  if (a->elem_bytes == 4) return launch_accept<uint32_t>(g, a, st);
+  if (a->elem_bytes == 2) return launch_accept<uint16_t>(g, a, st);
+  return launch_accept<uint8_t>(g, a, st);
 }
 
 // -------------------------------------------------------------- attention --
@@ -315,8 +336,7 @@ int launch_prompt(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMa
   constexpr int smem = SvSmem<DP, true>::kBytes;
   static SmemGrant grant;
   if (const int rc = grant(reinterpret_cast<const void*>(kern), smem)) return rc;
-  kern<<<blocks, kSvThreads, smem, st>>>(tq, tk, tv, g);
-  return launch_status();
+  return launch_dependent(kern, dim3(blocks), kSvThreads, smem, st, tq, tk, tv, g);
 }
 
 // The attention over a cache with items of kTileRows rows, then the join of
@@ -331,30 +351,17 @@ int launch_cache(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap
     auto kern = serving_attention_kernel<DP, T, true, kPair>;
     constexpr int smem = SvSmem<DP, kPair>::kBytes;
     if ((rc = grant(reinterpret_cast<const void*>(kern), smem))) return rc;
-    kern<<<blocks, kSvThreads, smem, st>>>(tq, tk, tv, g);
+    rc = launch_dependent(kern, dim3(blocks), kSvThreads, smem, st, tq, tk, tv, g);
   } else {
     auto kern = decode_attention_kernel<DP, T, kTileRows>;
     constexpr int smem = DcSmem<DP, kTileRows>::kBytes;
     if ((rc = grant(reinterpret_cast<const void*>(kern), smem))) return rc;
-    kern<<<blocks, kDcThreads, smem, st>>>(tk, tv, g);
+    rc = launch_dependent(kern, dim3(blocks), kDcThreads, smem, st, tk, tv, g);
   }
-  if ((rc = launch_status())) return rc;
-  // a programmatic dependent: its blocks are dispatched, and find their cut
-  // item, while the parts are still being computed
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(blocks, kSvJoinSplit<kTileRows>);
-  cfg.blockDim = dim3(kSvJoinThreads);
-  cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, attention_join_kernel<DP, T, kTileRows>, g) != cudaSuccess) {
-    cudaGetLastError();
-    return AKILI_E_LAUNCH;
-  }
-  return launch_status();
+  if (rc) return rc;
+  // (its blocks find their cut item while the parts are still being computed)
+  return launch_dependent(attention_join_kernel<DP, T, kTileRows>, dim3(blocks, kSvJoinSplit<kTileRows>),
+                          kSvJoinThreads, 0, st, g);
 }
 
 template <int DP, typename T>
