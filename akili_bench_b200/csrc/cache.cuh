@@ -99,10 +99,12 @@ __global__ void __launch_bounds__(kAcceptThreads) cache_accept_kernel(const Acce
       k_src[r] = -1;
       bool ok = x >= i && (i == 0 || x > acc[i - 1]) && s < cap;
       if (ok) {
-        const int ps = table[s / a.page_size], pd = table[d / a.page_size];
+        // (below 2^32: the sum of two ints)
+        const uint32_t us = static_cast<uint32_t>(s), ud = static_cast<uint32_t>(d), size = a.page_size;
+        const int ps = table[us / size], pd = table[ud / size];
         ok = ps >= 0 && ps < a.num_pages && pd >= 0 && pd < a.num_pages;
         if (ok && s != d) {
-          const long long os = s % a.page_size, od = d % a.page_size;
+          const long long os = us % size, od = ud % size;
           k_src[r] = ps * a.k_st[1] + os * a.k_st[2];
           k_dst[r] = pd * a.k_st[1] + od * a.k_st[2];
           v_src[r] = ps * a.v_st[1] + os * a.v_st[2];
@@ -120,7 +122,7 @@ __global__ void __launch_bounds__(kAcceptThreads) cache_accept_kernel(const Acce
       base += static_cast<long long>(x) * sizeof(U);
       const long long* src = is_v ? v_src : k_src;
       const long long* dst = is_v ? v_dst : k_dst;
-      constexpr int kBatch = 4;
+      constexpr int kBatch = 8;
       for (int r = 0; r < m; r += kBatch) {
         U held[kBatch];
         bool live[kBatch];

@@ -45,6 +45,23 @@ struct alignas(sizeof(T) * VEC) ValueVec {
   T v[VEC];
 };
 
+// Two values at a time.
+__device__ __forceinline__ float2 to_f32x2(const float* x) { return make_float2(x[0], x[1]); }
+__device__ __forceinline__ float2 to_f32x2(const __half* x) { return __half22float2(*reinterpret_cast<const __half2*>(x)); }
+__device__ __forceinline__ float2 to_f32x2(const __nv_bfloat16* x) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(x));
+}
+__device__ __forceinline__ void from_f32x2(float* y, float a, float b) {
+  y[0] = a;
+  y[1] = b;
+}
+__device__ __forceinline__ void from_f32x2(__half* y, float a, float b) {
+  *reinterpret_cast<__half2*>(y) = __floats2half2_rn(a, b);
+}
+__device__ __forceinline__ void from_f32x2(__nv_bfloat16* y, float a, float b) {
+  *reinterpret_cast<__nv_bfloat162*>(y) = __floats2bfloat162_rn(a, b);
+}
+
 struct RopeArgs {
   const void *q, *k, *v;
   void *q_out, *k_out, *v_out;  // append: k_out, v_out are the pages
@@ -101,11 +118,21 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
     const bool turn = u < turn_units;
     float c[VEC], s[VEC];
     if (turn) {
+      if constexpr (VEC % 4 == 0) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        c[i] = row[u * VEC + i];
-        s[i] = row[half + u * VEC + i] * a.sin_sign;
+        for (int i = 0; i < VEC; i += 4) {
+          *reinterpret_cast<float4*>(c + i) = *reinterpret_cast<const float4*>(row + u * VEC + i);
+          *reinterpret_cast<float4*>(s + i) = *reinterpret_cast<const float4*>(row + half + u * VEC + i);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          c[i] = row[u * VEC + i];
+          s[i] = row[half + u * VEC + i];
+        }
       }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) s[i] *= a.sin_sign;
     }
     // offsets of the unit's two vectors within a head
     int o0, o1;
@@ -139,31 +166,25 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
       V x0 = *reinterpret_cast<const V*>(src + o0);
       V x1 = *reinterpret_cast<const V*>(src + o1);
       if (rotate) {
-        if (a.interleaved) {
+        if constexpr (VEC == 1) {
+          const float y1 = to_f32(x0.v[0]), y2 = to_f32(x1.v[0]);
+          x0.v[0] = from_f32<T>(y1 * c[0] - y2 * s[0]);
+          x1.v[0] = from_f32<T>(y2 * c[0] + y1 * s[0]);
+        } else if (a.interleaved) {
           // x0 and x1 hold the pairs (0, 1), (2, 3), ... of 2 VEC values in a row
-          T* e = x0.v;
-          T* f = x1.v;
-          if constexpr (VEC == 1) {
-            const float y1 = to_f32(e[0]), y2 = to_f32(f[0]);
-            e[0] = from_f32<T>(y1 * c[0] - y2 * s[0]);
-            f[0] = from_f32<T>(y2 * c[0] + y1 * s[0]);
-          } else {
 #pragma unroll
-            for (int i = 0; i < VEC / 2; ++i) {
-              const float a1 = to_f32(e[2 * i]), a2 = to_f32(e[2 * i + 1]);
-              e[2 * i] = from_f32<T>(a1 * c[i] - a2 * s[i]);
-              e[2 * i + 1] = from_f32<T>(a2 * c[i] + a1 * s[i]);
-              const float b1 = to_f32(f[2 * i]), b2 = to_f32(f[2 * i + 1]);
-              f[2 * i] = from_f32<T>(b1 * c[VEC / 2 + i] - b2 * s[VEC / 2 + i]);
-              f[2 * i + 1] = from_f32<T>(b2 * c[VEC / 2 + i] + b1 * s[VEC / 2 + i]);
-            }
+          for (int i = 0; i < VEC / 2; ++i) {
+            const float2 y = to_f32x2(x0.v + 2 * i), z = to_f32x2(x1.v + 2 * i);
+            from_f32x2(x0.v + 2 * i, y.x * c[i] - y.y * s[i], y.y * c[i] + y.x * s[i]);
+            from_f32x2(x1.v + 2 * i, z.x * c[VEC / 2 + i] - z.y * s[VEC / 2 + i],
+                       z.y * c[VEC / 2 + i] + z.x * s[VEC / 2 + i]);
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float y1 = to_f32(x0.v[i]), y2 = to_f32(x1.v[i]);
-            x0.v[i] = from_f32<T>(y1 * c[i] - y2 * s[i]);
-            x1.v[i] = from_f32<T>(y2 * c[i] + y1 * s[i]);
+          for (int i = 0; i < VEC; i += 2) {
+            const float2 y = to_f32x2(x0.v + i), z = to_f32x2(x1.v + i);
+            from_f32x2(x0.v + i, y.x * c[i] - z.x * s[i], y.y * c[i + 1] - z.y * s[i + 1]);
+            from_f32x2(x1.v + i, z.x * c[i] + y.x * s[i], z.y * c[i + 1] + y.y * s[i + 1]);
           }
         }
       }
