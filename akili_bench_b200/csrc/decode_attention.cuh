@@ -81,20 +81,6 @@ __device__ __forceinline__ void lane_reduce(float (&v)[N], Op op) {
   }
 }
 
-// Barrier of the 128 softmax threads that returns whether any of them votes.
-__device__ __forceinline__ bool vote_barrier(uint32_t id, bool vote) {
-  uint32_t any;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, %2, 128, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(any)
-      : "r"(static_cast<uint32_t>(vote)), "r"(id)
-      : "memory");
-  return any != 0;
-}
-
 template <int N>
 __device__ __forceinline__ void tmem_ld_n(uint32_t taddr, float (&v)[N]) {
   if constexpr (N == 64) {
@@ -420,7 +406,7 @@ __global__ void __launch_bounds__(kDcThreads, 1)
         for (int n = 0; n < N; ++n) grow = grow || fmaf(s[n], sl, -m[n]) > 8.0f;
         // the P buffer's last reader, block g - 2
         if (g >= 2 && !mbar_wait(&ctl->pv_done[g & 1], ((g >> 1) - 1) & 1, kSiteFlashPV)) ctl->abort[g & 1] = 1;
-        grow = vote_barrier(kBar, grow);
+        grow = vote_barrier<128>(kBar, grow);
         if (ctl->abort[g & 1]) {
           alive = false;
           break;

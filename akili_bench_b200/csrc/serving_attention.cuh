@@ -29,12 +29,12 @@
 //                stream's previous block, then S_t = Q_t K^T of its next one
 //                (over the columns of that P_t; the MMAs run in order).
 //   2..9, 10..17 softmax of stream 0 and 1: two threads per row with 64 of a
-//                block's 128 scores each.  They swap their block maxima
-//                through shared memory behind a barrier of their two warps,
-//                keep the running maximum (rescaling O_t in TMEM only when it
-//                grows by more than 2^8: a stale maximum cancels in O / l) and
-//                write P = exp2(scale log2e s - m) over S_t in parts, each
-//                announced to the MMA warp on its own.
+//                block's 128 scores each.  The running maximum only matters
+//                where it grows by more than 2^8 (a stale one cancels in
+//                O / l), so their two warps vote behind one barrier a block
+//                and exchange maxima through shared memory, and rescale O_t,
+//                only then.  P = exp2(scale log2e s - m) goes over S_t in two
+//                parts, each announced to the MMA warp on its own.
 //   19           scheduler: finds the next piece of work, hands it to the
 //                others through a small ring, and loads its Q by TMA as soon
 //                as the last scores of the piece before are done.  A piece
@@ -448,6 +448,21 @@ __device__ __forceinline__ uint64_t mask_window(const unsigned int* row, int wor
   return v;
 }
 
+// Barrier of kThreads threads that returns whether any of them votes.
+template <int kThreads>
+__device__ __forceinline__ bool vote_barrier(uint32_t id, bool vote) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, %2, %3, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(static_cast<uint32_t>(vote)), "r"(id), "n"(kThreads)
+      : "memory");
+  return any != 0;
+}
+
 // ----------------------------------------------------------------- kernel --
 template <int DP, typename T, bool kPaged, bool kPair>
 __global__ void __maxnreg__(96)
@@ -457,7 +472,7 @@ __global__ void __maxnreg__(96)
   constexpr int kTileRows = (kPair ? 2 : 1) * kSvRows;
   constexpr int kStages = L::kStages;
   constexpr int kChunks = DP / 64;              // 64-column swizzle chunks
-  constexpr int kParts = DP >= 128 ? 4 : 2;     // parts in which P is announced
+  constexpr int kParts = 2;                     // in which P is announced (4: 3% slower, 1: 5%)
   constexpr int kPSteps = 4 / kParts;           // P.V K-steps per part and half
   constexpr int kPPairs = 8 * kPSteps;          // packed P columns per part and half
   constexpr uint32_t kColO = 256;
@@ -882,8 +897,7 @@ __global__ void __maxnreg__(96)
         if (!mbar_wait(&ctl->s_full[grp], s_cnt & 1, kSiteFlashS)) ctl->pair_abort[pair_id][events & 1] = 1;
         if (!warp_live) {
           // no row here: nothing reads these lanes of P
-          named_bar_sync(pair_bar, 64);
-          if constexpr (L::kXBufs == 1) named_bar_sync(pair_bar, 64);
+          vote_barrier<64>(pair_bar, false);
           if (ctl->pair_abort[pair_id][events & 1]) {
             alive = false;
             break;
@@ -922,20 +936,27 @@ __global__ void __maxnreg__(96)
         }
         const float pmax = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
                                  fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
-        float* xs = swap_slot(events);
-        xs[half * kSvRows + r] = pmax;
+        // One vote of the two warps (which also orders both halves' S loads
+        // before either's P stores); the maxima are exchanged only when some
+        // row's grows.
         tc_fence_before();
-        named_bar_sync(pair_bar, 64);
+        const bool any_grow = vote_barrier<64>(pair_bar, sl * pmax > m_use + 8.0f);
         tc_fence_after();
-        const float other = xs[(half ^ 1) * kSvRows + r];
-        if constexpr (L::kXBufs == 1) named_bar_sync(pair_bar, 64);
         if (ctl->pair_abort[pair_id][events & 1]) {
           alive = false;
           break;
         }
-        const float rmax = sl * fmaxf(pmax, other);
-        const bool grow = rmax > m_use + 8.0f;
-        const float m_new = grow ? rmax : m_use;
+        bool grow = false;
+        float m_new = m_use;
+        if (any_grow) {
+          float* xs = swap_slot(events);
+          xs[half * kSvRows + r] = pmax;
+          named_bar_sync(pair_bar, 64);
+          const float rmax = sl * fmaxf(pmax, xs[(half ^ 1) * kSvRows + r]);
+          if constexpr (L::kXBufs == 1) named_bar_sync(pair_bar, 64);
+          grow = rmax > m_use + 8.0f;
+          if (grow) m_new = rmax;
+        }
         const float alpha = grow ? exp2f(m_use - m_new) : 1.0f;  // 0 on the first block with a visible key
         if (i > 0 && __any_sync(0xffffffffu, grow)) {
           const uint32_t tO = tmem + lane_off + kColO + grp * 128 + half * (DP / 2);
