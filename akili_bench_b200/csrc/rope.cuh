@@ -65,6 +65,7 @@ __device__ __forceinline__ void from_f32x2(__nv_bfloat16* y, float a, float b) {
 struct RopeArgs {
   const void *q, *k, *v;
   void *q_out, *k_out, *v_out;  // append: k_out, v_out are the pages
+  void* k_copy;                 // append: optional, the rotated k by token
   const int* positions;
   const float* table;
   const long long* slots;  // append only
@@ -74,6 +75,7 @@ struct RopeArgs {
   float sin_sign;
   long long q_st[2], k_st[2], v_st[2], qo_st[2];
   long long ko_st[3], vo_st[3];  // page, token, head (akili_rope: 0, token, head)
+  long long kc_st[2];
 };
 
 // Threads of a block: `hl` head lanes of `ul` consecutive units each.  A unit
@@ -146,16 +148,17 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
     for (int h = blockIdx.y * hl + lane_h; h < heads; h += gridDim.y * hl) {
       const T* src;
       T* dst;
+      T* copy = nullptr;
       bool rotate = turn;
       if (h < a.q_heads) {
         src = static_cast<const T*>(a.q) + t * a.q_st[0] + h * a.q_st[1];
         dst = static_cast<T*>(a.q_out) + t * a.qo_st[0] + h * a.qo_st[1];
       } else {
-        if (kAppend && !store_kv) continue;
         int hk = h - a.q_heads;
         if (!kAppend || hk < a.k_heads) {
           src = static_cast<const T*>(a.k) + t * a.k_st[0] + hk * a.k_st[1];
           dst = static_cast<T*>(a.k_out) + page * a.ko_st[0] + in_page * a.ko_st[1] + hk * a.ko_st[2];
+          if (kAppend && a.k_copy != nullptr) copy = static_cast<T*>(a.k_copy) + t * a.kc_st[0] + hk * a.kc_st[1];
         } else {
           hk -= a.k_heads;
           src = static_cast<const T*>(a.v) + t * a.v_st[0] + hk * a.v_st[1];
@@ -188,8 +191,14 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a) {
           }
         }
       }
-      *reinterpret_cast<V*>(dst + o0) = x0;
-      *reinterpret_cast<V*>(dst + o1) = x1;
+      if (h < a.q_heads || store_kv) {
+        *reinterpret_cast<V*>(dst + o0) = x0;
+        *reinterpret_cast<V*>(dst + o1) = x1;
+      }
+      if (copy != nullptr) {
+        *reinterpret_cast<V*>(copy + o0) = x0;
+        *reinterpret_cast<V*>(copy + o1) = x1;
+      }
     }
   }
 }

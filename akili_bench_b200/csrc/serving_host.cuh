@@ -88,6 +88,7 @@ int run_rope(const akili_rope_arg_t* a, bool append, cudaStream_t st) {
   if (a->k_heads && (rc = check_aligned({a->k_addr}, es))) return rc;
   if (a->k_heads && !append && (rc = check_aligned({a->k_out_addr}, es))) return rc;
   if (a->k_heads && append && (rc = check_aligned({a->v_addr, a->k_pages_addr, a->v_pages_addr}, es))) return rc;
+  if (append && a->k_out_addr % es) return AKILI_E_ALIGN;
   if (append && (rc = check_aligned({a->slots_addr}, 8))) return rc;
   DevInfo di;
   if ((rc = device_info(&di))) return rc;
@@ -96,6 +97,7 @@ int run_rope(const akili_rope_arg_t* a, bool append, cudaStream_t st) {
   r.q_out = W(a->q_out_addr);
   r.k_out = W(append ? a->k_pages_addr : a->k_out_addr);
   r.v_out = W(a->v_pages_addr);
+  r.k_copy = append ? W(a->k_out_addr) : nullptr;
   r.positions = static_cast<const int*>(P(a->positions_addr));
   r.table = F(a->table_addr);
   r.slots = static_cast<const long long*>(P(a->slots_addr));
@@ -107,7 +109,7 @@ int run_rope(const akili_rope_arg_t* a, bool append, cudaStream_t st) {
   for (int i = 0; i < 2; ++i) {
     r.q_st[i] = a->q_stride[i]; r.k_st[i] = a->k_stride[i]; r.qo_st[i] = a->q_out_stride[i];
     r.v_st[i] = a->v_stride[i];
-    r.ko_st[i + 1] = a->k_out_stride[i];
+    r.ko_st[i + 1] = r.kc_st[i] = a->k_out_stride[i];
   }
   if (append)
     for (int i = 0; i < 3; ++i) { r.ko_st[i] = a->k_page_stride[i]; r.vo_st[i] = a->v_page_stride[i]; }
@@ -121,7 +123,8 @@ int run_rope(const akili_rope_arg_t* a, bool append, cudaStream_t st) {
     vec = vec && a->k_addr % 16 == 0 && all_multiples(a->k_stride, n);
     if (append)
       vec = vec && (a->v_addr | a->k_pages_addr | a->v_pages_addr) % 16 == 0 && all_multiples(a->v_stride, n) &&
-            all_multiples(a->k_page_stride, n) && all_multiples(a->v_page_stride, n);
+            all_multiples(a->k_page_stride, n) && all_multiples(a->v_page_stride, n) &&
+            (!a->k_out_addr || (a->k_out_addr % 16 == 0 && all_multiples(a->k_out_stride, n)));
     else
       vec = vec && a->k_out_addr % 16 == 0 && all_multiples(a->k_out_stride, n);
   }

@@ -189,7 +189,7 @@ PyObject* rope(PyObject* const* v) {
   return Py_BuildValue("(NN)", THPVariable_Wrap(q_out), THPVariable_Wrap(k_out));
 }
 
-// (q, k, v, positions, table, slots, k_pages, v_pages, interleaved, q_out, stream)
+// (q, k, v, positions, table, slots, k_pages, v_pages, interleaved, q_out, k_out, stream)
 PyObject* rope_append(PyObject* const* v) {
   akili_rope_arg_t a = {};
   const at::Tensor &q = tensor(v[0], "q"), &k = tensor(v[1], "k"), &val = tensor(v[2], "v"),
@@ -213,7 +213,14 @@ PyObject* rope_append(PyObject* const* v) {
   strides(a.v_stride, val);
   strides(a.k_page_stride, kp);
   strides(a.v_page_stride, vp);
-  if (const int rc = akili_rope_append(&a, stream_of(v[10]))) refuse("rope_append", rc);
+  if (v[10] != Py_None) {
+    const at::Tensor& k_out = tensor(v[10], "k_out");
+    values(q, k_out, "k_out");
+    shape_is(k_out, {k.size(0), k.size(1), k.size(2)}, "k_out");
+    a.k_out_addr = addr(k_out);
+    strides(a.k_out_stride, k_out);
+  }
+  if (const int rc = akili_rope_append(&a, stream_of(v[11]))) refuse("rope_append", rc);
   return THPVariable_Wrap(q_out);
 }
 
@@ -436,7 +443,7 @@ PyMethodDef method(const char* name) {
 }
 
 PyMethodDef methods[] = {method<rope, 9>("rope"),
-                         method<rope_append, 11>("rope_append"),
+                         method<rope_append, 12>("rope_append"),
                          method<rope_table, 9>("rope_table"),
                          method<prompt_attention, 10>("prompt_attention"),
                          method<tree_mask, 4>("tree_mask"),

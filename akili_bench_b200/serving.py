@@ -13,8 +13,8 @@ prompts and to decode over a paged key/value cache:
 Tensors are CUDA tensors on the current device, of any strides with a
 contiguous last axis; index tensors are int32 (slots int64).  Wrong types,
 shapes or devices raise TypeError or ValueError before the launch; the C
-entry's own refusals raise ``abi.AkiliError``.  Calls run on ``stream`` (default: the current stream)
-and do not synchronise.
+entry's own refusals raise ``abi.AkiliError``.  Calls run on ``stream``
+(default: the current stream) and do not synchronise.
 """
 from __future__ import annotations
 
@@ -83,12 +83,14 @@ def rope(q, k, positions, table, interleaved: bool = False, inverse: bool = Fals
 
 
 def rope_append(q, k, v, positions, table, slots, k_pages, v_pages, interleaved: bool = False, q_out=None,
-                stream=None):
+                k_out=None, stream=None):
     """`rope`, with the rotated k and v [tokens, k_heads, head_dim] written to row slots[token] = page *
     page_size + offset (int64; -1: padding, nothing is written) of k_pages/v_pages [num_pages, page_size,
-    k_heads, head_dim].  Returns the rotated q (q_out; may be q)."""
+    k_heads, head_dim].  k_out, if given, gets the rotated k as well (`prompt_attention` of the same prompt
+    reads it; it may be k).  Returns the rotated q (q_out; may be q)."""
     return _on(stream, q_out is not None,
-               _native.rope_append(q, k, v, positions, table, slots, k_pages, v_pages, interleaved, q_out, stream))
+               _native.rope_append(q, k, v, positions, table, slots, k_pages, v_pages, interleaved, q_out, k_out,
+                                   stream))
 
 
 def _attention_result(got, out, return_lse, stream):

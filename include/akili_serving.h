@@ -57,7 +57,7 @@ typedef struct {
   uint32_t rot_dim;       /* even, 0 < rot_dim <= head_dim */
   uint32_t max_positions; /* rows of the table */
   uint64_t q_addr, k_addr, q_out_addr;
-  uint64_t k_out_addr;     /* akili_rope only */
+  uint64_t k_out_addr;     /* akili_rope_append: optional, the rotated k once more (for a prompt's own attention) */
   uint64_t positions_addr; /* int32 [tokens] */
   uint64_t table_addr;     /* fp32 [max_positions, rot_dim]: rot_dim/2 cosines, then the sines */
   int64_t  q_stride[2], k_stride[2], q_out_stride[2], k_out_stride[2]; /* token, head */

@@ -192,6 +192,26 @@ def test_rope_append(dtype, heads_first, tokens, hq, hk, d, rot, page):
         assert torch.isnan(kf[rest]).all() and torch.isnan(vf[rest]).all()
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+def test_rope_append_keeps_the_rotated_keys_of_every_token(in_place):
+    g = gen(77)
+    q, k, v = (normal(g, (21, h, 64), BF16) for h in (4, 2, 2))
+    pages = torch.zeros(2, 16, 2, 64, dtype=BF16, device="cuda")
+    v_pages = torch.zeros_like(pages)
+    slots = torch.arange(21)
+    slots[5] = -1  # padding goes to no page, but is rotated
+    pos, table = torch.arange(21, dtype=torch.int32), normal(g, (30, 64), F32)
+    dev_k = k.cuda()
+    k_out = dev_k if in_place else torch.empty(2, 21, 64, dtype=BF16, device="cuda").transpose(0, 1)
+    ops.rope_append(q.cuda(), dev_k, v.cuda(), pos.cuda(), table.cuda(), slots.cuda(), pages, v_pages, k_out=k_out)
+    want, bound = ref.rotate(k, pos, table)
+    ref.assert_within(k_out, want, bound)
+    on = slots >= 0
+    flat = pages.view(-1, 2, 64)
+    assert torch.equal(flat[slots[on].cuda()], k_out[on.cuda()])
+    assert (flat[5] == 0).all() and (v_pages.view(-1, 2, 64)[5] == 0).all()
+
+
 def test_rope_append_skips_slots_outside_the_pages():
     q = torch.ones(2, 1, 8, dtype=F16, device="cuda")
     pages = torch.zeros(2, 4, 1, 8, dtype=F16, device="cuda")
