@@ -17,6 +17,10 @@
 // score passes the running maximum by more than 2^8 (a stale maximum cancels
 // in O / l): one barrier per block carries that vote, and the reduction and
 // the rescaling of O run only then.  Row sums stay per thread until the end.
+// What belongs to a row (maximum, factors, address, its visible keys as bit
+// words of a block) is worked out by one thread and read by all from shared
+// memory; with every thread doing so for itself a short item of 64 rows took
+// 36000 cycles.
 //
 // Warps: 0 key loads, 1 value loads (each issues its own ring's TMA boxes, one
 // per page part), 2 TMEM owner and MMA issuer, 3 loads the next item's Q, 4..7
@@ -42,8 +46,9 @@ struct DcSmem {
   // this memory: rows of O^T that nobody uses)
   static constexpr int kQOff = kVOff + kVStages * kKV;
   static constexpr int kPOff = kQOff + 2 * kQ;
-  static constexpr int kXOff = DP == 64 && 2 * (kQ + kP) < 16384 ? kQOff + 16384 : kPOff + 2 * kP;  // [4 warps][N] exchange
-  static constexpr int kCtlOff = kXOff + 4 * N * 4;
+  static constexpr int kXOff = DP == 64 && 2 * (kQ + kP) < 16384 ? kQOff + 16384 : kPOff + 2 * kP;
+  // by row: [4 warps] exchange, [4 x 32 keys] visible bits, maximum, factor
+  static constexpr int kCtlOff = kXOff + 10 * N * 4;
   static constexpr int kBytes = kCtlOff + 512;
   static_assert(kBytes <= 232448, "227 KB of shared memory per CTA");
 };
@@ -116,6 +121,9 @@ __global__ void __launch_bounds__(kDcThreads, 1)
   auto* ctl = reinterpret_cast<DcControl*>(smem + L::kCtlOff);
   static_assert(sizeof(DcControl) <= 512, "control block");
   float* xchg = reinterpret_cast<float*>(smem + L::kXOff);
+  uint32_t* visible = reinterpret_cast<uint32_t*>(xchg + 4 * N);
+  float* row_max = xchg + 8 * N;
+  float* factor = xchg + 9 * N;
   const uint32_t warp = warp_id();
   const uint32_t lane = lane_id();
 
@@ -354,19 +362,23 @@ __global__ void __launch_bounds__(kDcThreads, 1)
     const bool tree = a.mask != nullptr;
     uint32_t g = 0, item = 0;
     bool alive = true;
-    float m[N], l[N];
+    float l[N];
+    // lane_reduce's results -> the exchange
+    auto share = [&](const float (&v)[N]) {
+      if constexpr (N >= 32) {
+#pragma unroll
+        for (int i = 0; i < N / 32; ++i) xchg[wq * N + lane * (N / 32) + i] = v[i];
+      } else {
+        if (lane % (32 / N) == 0) xchg[wq * N + lane / (32 / N)] = v[0];
+      }
+    };
     for (; alive && have; ++item, have = next()) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        m[n] = -3.4028235e38f;  // "nothing seen": any finite score passes it
-        l[n] = 0.0f;
-      }
+      for (int n = 0; n < N; ++n) l[n] = 0.0f;
       const int row0 = pc.tile * N;
-      const int tok0 = row0 / a.group;
-      const int rem0 = row0 - tok0 * a.group;
       const int nrows = min(N, pc.s.n * a.group - row0);
       // keys that every row sees
-      const int common = tree ? pc.s.sure : min(pc.s.m, pc.s.sure + tok0 + 1);
+      const int common = tree ? pc.s.sure : min(pc.s.m, pc.s.sure + row0 / a.group + 1);
       for (int j = 0; j < pc.loads; ++j, ++g) {
         const int key0 = (pc.kb + j) * kSvKeys;
         if (!mbar_wait(&ctl->s_full[g & 1], (g >> 1) & 1, kSiteFlashS)) ctl->abort[g & 1] = 1;
@@ -374,92 +386,104 @@ __global__ void __launch_bounds__(kDcThreads, 1)
         float s[N];
         tmem_ld_n<N>(tbase + (g & 1) * N, s);
         if (key0 + kSvKeys > common) {
-          const int key = key0 + t;
-          const int node = key - pc.s.sure;
-          int tok = tok0, rem = rem0;
-          if (key < pc.s.m && tree && node >= 0) {
-#pragma unroll
-            for (int n = 0; n < N; ++n) {
-              bool see = false;
-              if (n < nrows && node / 32 < a.mask_words)
-                see = (a.mask[(pc.s.q0 + tok) * a.mask_stride + node / 32] >> (node & 31)) & 1;
-              if (!see) s[n] = -INFINITY;
-              if (++rem == a.group) {
-                rem = 0;
-                ++tok;
+          // the keys each row sees, 32 to a word
+          for (int x = t; x < 4 * N; x += 128) {
+            const int n = x % N, first = key0 + 32 * (x / N);
+            uint32_t word = 0;
+            if (n < nrows) {
+              const int tok = (row0 + n) / a.group;
+              const int nv = (tree ? pc.s.sure : min(pc.s.m, pc.s.sure + tok + 1)) - first;
+              word = nv <= 0 ? 0u : nv >= 32 ? ~0u : (1u << nv) - 1;
+              const int node = first - pc.s.sure, nodes = pc.s.m - pc.s.sure;
+              if (tree && node > -32 && node < nodes) {
+                uint32_t bits = static_cast<uint32_t>(mask_window(a.mask + (pc.s.q0 + tok) * a.mask_stride, a.mask_words, node));
+                if (nodes - node < 32) bits &= (1u << (nodes - node)) - 1;
+                word |= bits;
               }
             }
-          } else {
-            const int last = key >= pc.s.m ? INT32_MAX : tree ? -1 : node;  // tokens before it do not see the key
-#pragma unroll
-            for (int n = 0; n < N; ++n) {
-              if (tok < last) s[n] = -INFINITY;
-              if (++rem == a.group) {
-                rem = 0;
-                ++tok;
-              }
-            }
-          }
-        }
-        bool grow = false;
-#pragma unroll
-        for (int n = 0; n < N; ++n) grow = grow || fmaf(s[n], sl, -m[n]) > 8.0f;
-        // the P buffer's last reader, block g - 2
-        if (g >= 2 && !mbar_wait(&ctl->pv_done[g & 1], ((g >> 1) - 1) & 1, kSiteFlashPV)) ctl->abort[g & 1] = 1;
-        grow = vote_barrier<128>(kBar, grow);
-        if (ctl->abort[g & 1]) {
-          alive = false;
-          break;
-        }
-        if (grow) {
-          float mx[N];
-#pragma unroll
-          for (int n = 0; n < N; ++n) mx[n] = s[n];
-          lane_reduce<N>(mx, [](float x, float y) { return fmaxf(x, y); });
-          if constexpr (N >= 32) {
-#pragma unroll
-            for (int i = 0; i < N / 32; ++i) xchg[wq * N + lane * (N / 32) + i] = mx[i];
-          } else {
-            if (lane % (32 / N) == 0) xchg[wq * N + lane / (32 / N)] = mx[0];
+            visible[x] = word;
           }
           named_bar_sync(kBar, 128);
-          float alpha[N];
 #pragma unroll
-          for (int n = 0; n < N; ++n) {
-            const float top = sl * fmaxf(fmaxf(xchg[n], xchg[N + n]), fmaxf(xchg[2 * N + n], xchg[3 * N + n]));
-            const float next_m = top > m[n] + 8.0f ? top : m[n];
-            alpha[n] = exp2f(m[n] - next_m);
-            l[n] *= alpha[n];
-            m[n] = next_m;
+          for (int n = 0; n < N; n += 4) {
+            const uint4 w = *reinterpret_cast<const uint4*>(visible + wq * N + n);
+            if (!((w.x >> lane) & 1)) s[n] = -INFINITY;
+            if (!((w.y >> lane) & 1)) s[n + 1] = -INFINITY;
+            if (!((w.z >> lane) & 1)) s[n + 2] = -INFINITY;
+            if (!((w.w >> lane) & 1)) s[n + 3] = -INFINITY;
           }
-          if (j > 0) {
-            // O holds the blocks up to g - 1 once their products are done
-            if (!mbar_wait(&ctl->pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, kSiteFlashPV)) ctl->abort[g & 1] = 1;
-            tc_fence_after();
-            const uint32_t to = tbase + kColO + (item & 1) * N;
+        }
+        // the P buffer's last reader, block g - 2
+        if (g >= 2 && !mbar_wait(&ctl->pv_done[g & 1], ((g >> 1) - 1) & 1, kSiteFlashPV)) ctl->abort[g & 1] = 1;
+        bool grow = true;  // an item's first block brings the maxima
+        if (j > 0) {
+          float over = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < N; c += 8) {
-              uint32_t e[8];
-              tmem_ld8(to + c, e);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) e[i] = __float_as_uint(__uint_as_float(e[i]) * alpha[c + i]);
-              tmem_st8(to + c, e);
-            }
+          for (int n = 0; n < N; n += 4) {
+            const float4 m = *reinterpret_cast<const float4*>(row_max + n);
+            over = fmaxf(over, fmaxf(fmaxf(fmaf(s[n], sl, -m.x), fmaf(s[n + 1], sl, -m.y)),
+                                     fmaxf(fmaf(s[n + 2], sl, -m.z), fmaf(s[n + 3], sl, -m.w))));
           }
-          named_bar_sync(kBar, 128);  // the exchange has been read; a wait that gave up is seen
+          grow = vote_barrier<128>(kBar, over > 8.0f);
           if (ctl->abort[g & 1]) {
             alive = false;
             break;
           }
         }
+        if (grow) {
+          {
+            float mx[N];
+#pragma unroll
+            for (int n = 0; n < N; ++n) mx[n] = s[n];
+            lane_reduce<N>(mx, [](float x, float y) { return fmaxf(x, y); });
+            share(mx);
+          }
+          named_bar_sync(kBar, 128);
+          if (t < N) {
+            // "nothing seen" is the lowest finite value: any finite score passes it
+            const float old = j > 0 ? row_max[t] : -3.4028235e38f;
+            const float top = sl * fmaxf(fmaxf(xchg[t], xchg[N + t]), fmaxf(xchg[2 * N + t], xchg[3 * N + t]));
+            const float now = top > old + 8.0f ? top : old;
+            row_max[t] = now;
+            factor[t] = exp2f(old - now);
+          }
+          // O holds the blocks up to g - 1 once their products are done
+          if (j > 0 && !mbar_wait(&ctl->pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, kSiteFlashPV)) ctl->abort[g & 1] = 1;
+          named_bar_sync(kBar, 128);
+          if (ctl->abort[g & 1]) {
+            alive = false;
+            break;
+          }
+          if (j > 0) {
+            tc_fence_after();
+            const uint32_t to = tbase + kColO + (item & 1) * N;
+#pragma unroll
+            for (int c = 0; c < N; c += 8) {
+              float f[8];
+              *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(factor + c);
+              *reinterpret_cast<float4*>(f + 4) = *reinterpret_cast<const float4*>(factor + c + 4);
+              uint32_t e[8];
+              tmem_ld8(to + c, e);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                l[c + i] *= f[i];
+                e[i] = __float_as_uint(__uint_as_float(e[i]) * f[i]);
+              }
+              tmem_st8(to + c, e);
+            }
+          }
+        }
         uint8_t* prow = smem + L::kPOff + (g & 1) * L::kP + t * (2 * N);
 #pragma unroll
         for (int u = 0; u < N / 8; ++u) {
+          float m[8];
+          *reinterpret_cast<float4*>(m) = *reinterpret_cast<const float4*>(row_max + u * 8);
+          *reinterpret_cast<float4*>(m + 4) = *reinterpret_cast<const float4*>(row_max + u * 8 + 4);
           uint32_t e[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int n = u * 8 + 2 * i;
-            const float p0 = ex2_mufu(fmaf(s[n], sl, -m[n])), p1 = ex2_mufu(fmaf(s[n + 1], sl, -m[n + 1]));
+            const float p0 = ex2_mufu(fmaf(s[n], sl, -m[2 * i])), p1 = ex2_mufu(fmaf(s[n + 1], sl, -m[2 * i + 1]));
             l[n] += p0;
             l[n + 1] += p1;
             e[i] = pack2<T>(p0, p1);
@@ -474,51 +498,58 @@ __global__ void __launch_bounds__(kDcThreads, 1)
       }
       // ---- output
       if (!alive) break;
-      if (!mbar_wait(&ctl->o_full[item & 1], (item >> 1) & 1, kSiteFlashPV)) ctl->abort[g & 1] = 1;
       lane_reduce<N>(l, [](float x, float y) { return x + y; });
-      if constexpr (N >= 32) {
-#pragma unroll
-        for (int i = 0; i < N / 32; ++i) xchg[wq * N + lane * (N / 32) + i] = l[i];
-      } else {
-        if (lane % (32 / N) == 0) xchg[wq * N + lane / (32 / N)] = l[0];
-      }
+      share(l);
+      if (!mbar_wait(&ctl->o_full[item & 1], (item >> 1) & 1, kSiteFlashPV)) ctl->abort[g & 1] = 1;
       named_bar_sync(kBar, 128);
       if (ctl->abort[g & 1]) {
         alive = false;
         break;
       }
+      float* slot = pc.part < 0 ? nullptr : a.parts + static_cast<size_t>(pc.part) * N * (DP + 2);
+      if (t < nrows) {
+        const float sum = (xchg[t] + xchg[N + t]) + (xchg[2 * N + t] + xchg[3 * N + t]);
+        const float m = sum != 0.0f ? row_max[t] : -INFINITY;
+        factor[t] = sum != 0.0f ? 1.0f / sum : 0.0f;
+        if (slot != nullptr) {
+          slot[N * DP + t] = m;
+          slot[N * (DP + 1) + t] = sum;
+        } else if (a.lse != nullptr) {
+          const int tok = (row0 + t) / a.group;
+          a.lse[(pc.s.q0 + tok) * static_cast<long long>(a.q_heads) + pc.hk * a.group + row0 + t - tok * a.group] =
+              (m + log2f(sum)) * 0.6931471805599453f;
+        }
+      }
       tc_fence_after();
       float o[N];
       tmem_ld_n<N>(tbase + kColO + (item & 1) * N, o);
       tc_fence_before();
-      __syncwarp();
+      named_bar_sync(kBar, 128);
       if (lane == 0) mbar_arrive(&ctl->o_empty[item & 1]);
-      float* slot = pc.part < 0 ? nullptr : a.parts + static_cast<size_t>(pc.part) * N * (DP + 2);
-      int tok = tok0, rem = rem0;
+      if (slot != nullptr) {
+        if (t < DP) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        if (n >= nrows) break;
-        const float sum = (xchg[n] + xchg[N + n]) + (xchg[2 * N + n] + xchg[3 * N + n]);
-        const long long qrow = pc.s.q0 + tok;
-        const int head = pc.hk * a.group + rem;
-        if (slot != nullptr) {
-          if (t < DP) slot[n * DP + t] = sum != 0.0f ? o[n] : 0.0f;
-          if (t == n) {
-            slot[N * DP + n] = sum != 0.0f ? m[n] : -INFINITY;
-            slot[N * (DP + 1) + n] = sum;
-          }
-        } else {
-          if (t < a.head_dim)
-            static_cast<T*>(a.o)[qrow * a.o_st[0] + head * a.o_st[1] + t] = from_f32<T>(sum != 0.0f ? o[n] * (1.0f / sum) : 0.0f);
-          if (t == n && a.lse != nullptr)
-            a.lse[qrow * a.q_heads + head] = sum != 0.0f ? (m[n] + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+          for (int n = 0; n < N; ++n)
+            if (n < nrows) slot[n * DP + t] = o[n];
         }
-        if (++rem == a.group) {
-          rem = 0;
-          ++tok;
+      } else if (t < a.head_dim) {
+        int rem = row0 % a.group;
+        T* out = static_cast<T*>(a.o) + (pc.s.q0 + row0 / a.group) * a.o_st[0] + (pc.hk * a.group + rem) * a.o_st[1] + t;
+        const long long next_tok = a.o_st[0] - (a.group - 1) * a.o_st[1];  // from a token's last head to the next one's first
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          if (n < nrows) {
+            const float f = factor[n];
+            *out = from_f32<T>(f != 0.0f ? o[n] * f : 0.0f);
+            if (++rem == a.group) {
+              rem = 0;
+              out += next_tok;
+            } else {
+              out += a.o_st[1];
+            }
+          }
         }
       }
-      named_bar_sync(kBar, 128);  // the sums have been read
     }
   }
 
