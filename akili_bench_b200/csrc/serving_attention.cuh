@@ -123,9 +123,14 @@ __device__ __forceinline__ SvSeq sv_sequence(const ServingArgs& a, int b, bool* 
 struct SvPiece {
   SvSeq s;
   int b, hk, tile;
-  int kb, loads;  // first key block, blocks
-  int part;       // slot of the workspace, or -1: the whole item
+  int kb, loads;    // first key block, blocks
+  int part;         // slot of the workspace, or -1: the whole item
+  long long first;  // place of the item's first block on the line
 };
+
+// An item's start and end take about as long as this many blocks, and count as
+// such on the line that is cut into shares (before its first block).
+constexpr int kSvItemCost = 2;
 
 // A CTA's share of the line of key blocks.  kTileRows: rows of an item, 128
 // or 256 of the row forms, 16 to 64 of the few-row form (whose tiles hold
@@ -147,38 +152,42 @@ struct SvWalk {
       tiles = (s.n * a.group + kTileRows - 1) / kTileRows;
     }
     blocks = (s.m + kSvKeys - 1) / kSvKeys;
-    size = static_cast<long long>(a.head_groups) * tiles * blocks;
+    size = static_cast<long long>(a.head_groups) * tiles * (blocks > 0 ? blocks + kSvItemCost : 0);
   }
   __device__ __forceinline__ bool next(const ServingArgs& a, int cta, SvPiece& p) {
-    if (pos >= end) return false;
-    while (off >= size) {
-      off -= size;
-      if (++b >= a.batch) return false;
-      bool clamped;
-      load(a, &clamped);
+    while (pos < end) {
+      while (off >= size) {
+        off -= size;
+        if (++b >= a.batch) return false;
+        bool clamped;
+        load(a, &clamped);
+      }
+      const int units = blocks + kSvItemCost;
+      long long item;
+      int at;  // unit within the item
+      if ((off >> 32) == 0) {  // (a 64-bit division costs some 100 cycles more)
+        const uint32_t i = static_cast<uint32_t>(off) / static_cast<uint32_t>(units);
+        item = i;
+        at = static_cast<int>(static_cast<uint32_t>(off) - i * static_cast<uint32_t>(units));
+        p.hk = static_cast<int>(i / static_cast<uint32_t>(tiles));
+      } else {
+        item = off / units;
+        at = static_cast<int>(off - item * units);
+        p.hk = static_cast<int>(item / tiles);
+      }
+      const int take = static_cast<int>(min(static_cast<long long>(units - at), end - pos));
+      p.s = s;
+      p.b = b;
+      p.tile = static_cast<int>(item - static_cast<long long>(p.hk) * tiles);
+      p.kb = max(at - kSvItemCost, 0);
+      p.loads = max(at + take - kSvItemCost, 0) - p.kb;
+      p.part = p.loads == blocks ? -1 : 2 * cta + (pos == begin ? 0 : 1);
+      p.first = pos - at + kSvItemCost;
+      pos += take;
+      off += take;
+      if (p.loads > 0) return true;  // (a share may end before the item's first block)
     }
-    long long item;
-    int kb;
-    if ((off >> 32) == 0) {  // (a 64-bit division costs some 100 cycles more)
-      const uint32_t i = static_cast<uint32_t>(off) / static_cast<uint32_t>(blocks);
-      item = i;
-      kb = static_cast<int>(static_cast<uint32_t>(off) - i * static_cast<uint32_t>(blocks));
-      p.hk = static_cast<int>(i / static_cast<uint32_t>(tiles));
-    } else {
-      item = off / blocks;
-      kb = static_cast<int>(off - item * blocks);
-      p.hk = static_cast<int>(item / tiles);
-    }
-    const int take = static_cast<int>(min(static_cast<long long>(blocks - kb), end - pos));
-    p.s = s;
-    p.b = b;
-    p.tile = static_cast<int>(item - static_cast<long long>(p.hk) * tiles);
-    p.kb = kb;
-    p.loads = take;
-    p.part = take == blocks ? -1 : 2 * cta + (pos == begin ? 0 : 1);
-    pos += take;
-    off += take;
-    return true;
+    return false;
   }
 };
 
@@ -256,56 +265,83 @@ __device__ __forceinline__ bool sv_share(const ServingArgs& a, int cta, int ctas
   return false;
 }
 
-// Prompts: block `id` of the grid -> (sequence, head group, tile pair), one
-// warp; false past the last.  chunk_heads head groups of all sequences are
-// taken together (their keys and values fit in L2 then), within them the tile
-// pairs level by level from the last (the one with the most keys under a
-// causal mask) to the first, so that the longest start earliest.
-__device__ __forceinline__ int sv_levels(const ServingArgs& a, int b) {
-  if (b >= a.batch) return 0;
-  const int q0 = min(max(a.cu_q[b], 0), a.total_q);
-  const int n = min(max(a.cu_q[b + 1], q0), a.total_q) - q0;
-  return (n + 2 * a.tile_tokens - 1) / (2 * a.tile_tokens);
-}
+// Prompts: block `id` of the grid -> (sequence, head group, tile or tile
+// pair), one warp; false past the last.  chunk_heads head groups of all
+// sequences are taken together (their keys and values fit in L2 then), within
+// them the tiles level by level from the last (the one with the most keys
+// under a causal mask) to the first, so that the longest start earliest.
+template <bool kPair>
 struct SvPromptLine {
-  int mine;   // levels of sequence `lane`
-  int top;    // most levels of any sequence
-  int tiles;  // tile pairs of a head group
-  __device__ __forceinline__ int at_least(const ServingArgs& a, int l) const {  // tile pairs of level l and above
-    int c = max(mine - l, 0);
-    for (int b0 = 32; b0 < a.batch; b0 += 32) c += max(sv_levels(a, b0 + static_cast<int>(lane_id())) - l, 0);
+  SvSeq mine;   // sequence `lane`
+  int levels;   // its tiles (tile pairs)
+  int top;      // most tiles of any sequence
+  int tiles;    // of a head group
+  __device__ __forceinline__ int levels_of(const ServingArgs& a, const SvSeq& s) const {
+    const int per = (kPair ? 2 : 1) * a.tile_tokens;
+    return (s.n + per - 1) / per;
+  }
+  __device__ __forceinline__ int levels_at(const ServingArgs& a, int b) const {
+    bool clamped;
+    return b < a.batch ? levels_of(a, sv_sequence<false>(a, b, &clamped)) : 0;
+  }
+  __device__ __forceinline__ int at_least(const ServingArgs& a, int l) const {  // tiles of level l and above
+    int c = max(levels - l, 0);
+    for (int b0 = 32; b0 < a.batch; b0 += 32) c += max(levels_at(a, b0 + static_cast<int>(lane_id())) - l, 0);
     return __reduce_add_sync(0xffffffffu, c);
   }
   __device__ __forceinline__ void load(const ServingArgs& a) {
-    mine = sv_levels(a, static_cast<int>(lane_id()));
-    top = mine;
-    for (int b0 = 32; b0 < a.batch; b0 += 32) top = max(top, sv_levels(a, b0 + static_cast<int>(lane_id())));
+    const int b = static_cast<int>(lane_id());
+    levels = 0;
+    if (b < a.batch) {
+      bool clamped;
+      mine = sv_sequence<false>(a, b, &clamped);
+      levels = levels_of(a, mine);
+    }
+    top = levels;
+    for (int b0 = 32; b0 < a.batch; b0 += 32) top = max(top, levels_at(a, b0 + b));
     top = __reduce_max_sync(0xffffffffu, top);
     tiles = at_least(a, 0);
   }
   // (the grid has fewer than 2^31 blocks, so 32 bits hold every count)
-  __device__ __forceinline__ bool find(const ServingArgs& a, uint32_t id, int* b_out, int* hk, int* level) const {
+  __device__ __forceinline__ bool find(const ServingArgs& a, uint32_t id, SvPiece& p) const {
     const uint32_t all = static_cast<uint32_t>(tiles);
     if (tiles == 0 || id / all >= static_cast<uint32_t>(a.head_groups)) return false;
     const uint32_t per = all * static_cast<uint32_t>(a.chunk_heads);  // of a chunk
     const uint32_t chunk = id / per, rem = id - chunk * per;
     const uint32_t heads = min(a.chunk_heads, a.head_groups - static_cast<int>(chunk) * a.chunk_heads);
     const int x = static_cast<int>(rem / heads);
-    *hk = static_cast<int>(chunk) * a.chunk_heads + static_cast<int>(rem - static_cast<uint32_t>(x) * heads);
-    int lo = 0, hi = top - 1;  // the last level with more than x tile pairs at or above it
+    p.hk = static_cast<int>(chunk) * a.chunk_heads + static_cast<int>(rem - static_cast<uint32_t>(x) * heads);
+    int lo = 0, hi = top - 1;  // the last level with more than x tiles at or above it
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (at_least(a, mid) > x) lo = mid;
       else hi = mid - 1;
     }
-    *level = lo;
+    p.tile = lo;
     int left = x - at_least(a, lo + 1);
+    const uint32_t lane = lane_id();
     for (int b0 = 0; b0 < a.batch; b0 += 32) {
-      const int levels = b0 == 0 ? mine : sv_levels(a, b0 + static_cast<int>(lane_id()));
-      const unsigned on = __ballot_sync(0xffffffffu, levels > lo);
+      SvSeq s = mine;
+      int l = levels;
+      if (b0 > 0) {
+        l = 0;
+        if (b0 + static_cast<int>(lane) < a.batch) {
+          bool clamped;
+          s = sv_sequence<false>(a, b0 + lane, &clamped);
+          l = levels_of(a, s);
+        }
+      }
+      const unsigned on = __ballot_sync(0xffffffffu, l > lo);
       const int c = __popc(on);
       if (left < c) {
-        *b_out = b0 + __fns(on, 0, left + 1);
+        const unsigned hit = __ballot_sync(0xffffffffu, l > lo && __popc(on & ((1u << lane) - 1)) == left);
+        const int at = __ffs(hit) - 1;
+        p.b = b0 + at;
+        p.s.q0 = __shfl_sync(0xffffffffu, s.q0, at);
+        p.s.n = __shfl_sync(0xffffffffu, s.n, at);
+        p.s.k0 = __shfl_sync(0xffffffffu, s.k0, at);
+        p.s.m = __shfl_sync(0xffffffffu, s.m, at);
+        p.s.sure = __shfl_sync(0xffffffffu, s.sure, at);
         return true;
       }
       left -= c;
@@ -525,7 +561,7 @@ __global__ void __maxnreg__(96)
   griddep_wait();
   if constexpr (kPaged) griddep_launch_dependents();
   // the scheduler finds its place meanwhile
-  SvPromptLine line;
+  SvPromptLine<kPair> line;
   SvWalk<kTileRows> walk;
   bool more = true;
   if (warp == 19) {
@@ -578,10 +614,8 @@ __global__ void __maxnreg__(96)
         }
         p.kb = 0;
         p.part = -1;
-        more = more && line.find(a, id, &p.b, &p.hk, &p.tile);
+        more = more && line.find(a, id, p);
         if (more) {
-          bool clamped;
-          p.s = sv_sequence<false>(a, p.b, &clamped);
           if (lane == 0) {
             mbar_expect_tx(&ctl->cancel, 16);
             request_block(&ctl->cancelled, &ctl->cancel);
@@ -618,6 +652,10 @@ __global__ void __maxnreg__(96)
         loads = max(n[0], n[1]);
       } else {
         loads = p.loads;
+        if constexpr (!kPaged) {
+          const int keys = a.causal ? max(min(p.s.m, p.s.sure + min(p.s.n, tok0 + a.tile_tokens)), 0) : p.s.m;
+          loads = (keys + kSvKeys - 1) / kSvKeys;
+        }
         n[0] = (loads + 1) >> 1;
         n[1] = loads >> 1;
       }
@@ -826,6 +864,7 @@ __global__ void __maxnreg__(96)
           }
         }
       } else {
+        if (loads == 0) continue;
         wait(&ctl->q_full[0], q_cnt[0]++ & 1, kSiteFlashQ);
         for (int j = 0; j < loads + 2 && ok; ++j) {
 #pragma unroll
@@ -1164,12 +1203,10 @@ __global__ void __launch_bounds__(kSvJoinThreads) attention_join_kernel(const __
     if (lane == 0) {
       parts = 0;
       SvPiece p;
-      while (work) {
-        const long long start = w.pos;
-        if (!w.next(a, blockIdx.x, p)) break;
+      while (work && w.next(a, blockIdx.x, p)) {
         if (p.part < 0 || p.kb != 0) continue;  // whole, or the end of an earlier share's item
         // starts here and is cut by the end of the share
-        const long long last = (start + w.blocks - 1) / quota;
+        const long long last = (p.first + w.blocks - 1) / quota;
         from = blockIdx.x;
         parts = static_cast<int>(last) - blockIdx.x + 1;
         slot0 = p.part;
