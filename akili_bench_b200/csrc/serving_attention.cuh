@@ -129,8 +129,10 @@ struct SvPiece {
 };
 
 // An item's start and end take about as long as this many blocks, and count as
-// such on the line that is cut into shares (before its first block).
-constexpr int kSvItemCost = 2;
+// such on the line that is cut into shares (before its first block).  25 drawn
+// batches, geometric mean: 1 block 26.7 us, 2 25.6, 3 25.4, 4 24.0, 6 23.9; 16
+// long drafted trees: 77.5, 77.8, 78.8, 80.5, 84.6.
+constexpr int kSvItemCost = 4;
 
 // A CTA's share of the line of key blocks.  kTileRows: rows of an item, 128
 // or 256 of the row forms, 16 to 64 of the few-row form (whose tiles hold

@@ -275,6 +275,15 @@ int check_heads(uint32_t dtype, uint32_t hq, uint32_t hk, uint32_t d, float scal
   return AKILI_OK;
 }
 
+// The tile loads need positive strides (a broadcast axis has 0); the stride of
+// an axis of one entry is never used.
+template <size_t n>
+bool loadable(const int64_t (&stride)[n], const uint64_t (&extent)[n]) {
+  for (size_t i = 0; i < n; ++i)
+    if (extent[i] > 1 && stride[i] <= 0) return false;
+  return true;
+}
+
 float scale_log2_of(float scale, uint32_t d) {
   return (scale != 0.0f ? scale : 1.0f / std::sqrt(static_cast<float>(d))) * 1.4426950408889634f;
 }
@@ -409,6 +418,9 @@ int run_prompt_attention(const akili_prompt_attention_arg_t* a, cudaStream_t st)
   if (!all_multiples(a->q_stride, 8) || !all_multiples(a->k_stride, 8) || !all_multiples(a->v_stride, 8) ||
       !all_multiples(a->o_stride, 8))
     return AKILI_E_ALIGN;
+  if (!loadable(a->q_stride, {a->total_q, a->q_heads}) || !loadable(a->k_stride, {a->total_k, a->kv_heads}) ||
+      !loadable(a->v_stride, {a->total_k, a->kv_heads}))
+    return AKILI_E_SHAPE;
   DevInfo di;
   if ((rc = device_info(&di))) return rc;
   const uint64_t group = a->q_heads / a->kv_heads;
@@ -485,6 +497,10 @@ int run_tree_attention(const akili_tree_attention_arg_t* a, cudaStream_t st) {
   if (!all_multiples(a->q_stride, 8) || !all_multiples(a->o_stride, 8) || !all_multiples(a->k_page_stride, 8) ||
       !all_multiples(a->v_page_stride, 8))
     return AKILI_E_ALIGN;
+  if (!loadable(a->q_stride, {a->total_q, a->q_heads}) ||
+      !loadable(a->k_page_stride, {a->num_pages, a->page_size, a->kv_heads}) ||
+      !loadable(a->v_page_stride, {a->num_pages, a->page_size, a->kv_heads}))
+    return AKILI_E_SHAPE;
   DevInfo di;
   if ((rc = device_info(&di))) return rc;
   Mode md;

@@ -127,7 +127,7 @@ typedef struct {
   uint64_t q_addr, k_addr, v_addr, o_addr;
   uint64_t lse_addr;              /* optional fp32 [total_q, q_heads]: log of the row's sum of exponentials */
   uint64_t cu_q_addr, cu_k_addr;  /* int32 [batch + 1], ascending from 0 */
-  int64_t  q_stride[2], k_stride[2], v_stride[2], o_stride[2]; /* token, head; multiples of 8 */
+  int64_t  q_stride[2], k_stride[2], v_stride[2], o_stride[2]; /* token, head; multiples of 8, positive */
 } akili_prompt_attention_arg_t;
 
 int akili_prompt_attention(const akili_prompt_attention_arg_t* arg, akili_stream_t stream);
@@ -159,8 +159,8 @@ typedef struct {
   uint64_t cu_q_addr;         /* int32 [batch + 1], ascending from 0 */
   uint64_t mask_addr;         /* optional int32 [total_q, mask_words] */
   uint64_t workspace, workspace_bytes; /* optional; akili_tree_attention_workspace() bytes, 256-byte aligned */
-  int64_t  q_stride[2], o_stride[2];           /* token, head; multiples of 8 */
-  int64_t  k_page_stride[3], v_page_stride[3]; /* page, token, head; multiples of 8 */
+  int64_t  q_stride[2], o_stride[2];           /* token, head; multiples of 8, positive */
+  int64_t  k_page_stride[3], v_page_stride[3]; /* page, token, head; multiples of 8, positive */
   int64_t  page_table_stride, mask_stride;     /* row strides */
 } akili_tree_attention_arg_t;
 

@@ -264,6 +264,42 @@ def test_prompt_attention(dtype, causal, case):
     check_prompt(q, k, v, qlens, klens, causal, got, lse)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("hq,hk,d", [(16, 8, 128), (16, 16, 64), (28, 4, 80), (48, 48, 128)])
+def test_prompt_attention_with_more_tiles_than_sms(dtype, causal, hq, hk, d):
+    """Two tiles a CTA, blocks taken over from the rest of the grid (small batches have one tile a CTA)."""
+    g = gen(hq + d)
+    qlens, klens = [420, 1, 0, 333, 130, 64], [500, 33, 7, 333, 129, 64]
+    q, k, v = normal(g, (sum(qlens), hq, d), dtype), normal(g, (sum(klens), hk, d), dtype), \
+        normal(g, (sum(klens), hk, d), dtype)
+    got, lse = ops.prompt_attention(q.cuda(), k.cuda(), v.cuda(), prefix(qlens).cuda(), prefix(klens).cuda(),
+                                    causal=causal, return_lse=True)
+    check_prompt(q, k, v, qlens, klens, causal, got, lse)
+
+
+def test_prompt_attention_without_any_key():
+    q = torch.ones(130, 4, 64, dtype=F16, device="cuda")
+    none = torch.empty(0, 2, 64, dtype=F16, device="cuda")
+    for causal in (True, False):
+        got, lse = ops.prompt_attention(q, none, none, i32([0, 100, 130]).cuda(), i32([0, 0, 0]).cuda(), causal=causal,
+                                        return_lse=True)
+        assert (got == 0).all() and (lse == -math.inf).all()
+
+
+def test_attention_refuses_broadcast_strides():
+    """An expanded axis has stride 0, which the tile loads cannot address."""
+    q = torch.ones(8, 4, 64, dtype=F16, device="cuda")
+    k = torch.ones(8, 1, 64, dtype=F16, device="cuda").expand(8, 4, 64)
+    with pytest.raises(abi.AkiliError) as e:
+        ops.prompt_attention(q, k, q, i32([0, 8]).cuda())
+    assert e.value.code == abi.E_SHAPE
+    pages = torch.ones(1, 8, 1, 64, dtype=F16, device="cuda").expand(2, 8, 2, 64)
+    with pytest.raises(abi.AkiliError) as e:
+        ops.tree_attention(q, pages, pages, i32([[0, 1]]).cuda(), i32([8]).cuda(), i32([0, 8]).cuda())
+    assert e.value.code == abi.E_SHAPE
+
+
 def test_prompt_attention_large_scores_and_scale():
     """Rising scores (the running maximum moves in every block) and scores in the hundreds."""
     g = gen(3)

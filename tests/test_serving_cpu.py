@@ -105,12 +105,13 @@ ATTENTION = [
     ({"batch": 0}, abi.E_SHAPE), ({"total_q": (1 << 30) + 1}, abi.E_SHAPE), ({"total_q": 0, "q_addr": 0}, abi.OK),
     ({"q_addr": 0}, abi.E_NULL_ARG), ({"o_addr": 0}, abi.E_NULL_ARG), ({"q_addr": A + 8}, abi.E_ALIGN),
     ({"lse_addr": A + 2}, abi.E_ALIGN), ({"cu_q_addr": 0}, abi.E_NULL_ARG), ({"q_stride_token": 516}, abi.E_ALIGN),
-    ({"o_stride_head": 4}, abi.E_ALIGN)]
+    ({"o_stride_head": 4}, abi.E_ALIGN), ({"q_stride_head": 0}, abi.E_SHAPE), ({"q_stride_token": -512}, abi.E_SHAPE)]
 
 
 @pytest.mark.parametrize("change,want", ATTENTION + [
     ({"causal": 2}, abi.E_UNSUPPORTED), ({"k_addr": 0}, abi.E_NULL_ARG), ({"cu_k_addr": 0}, abi.E_NULL_ARG),
-    ({"cu_k_addr": A + 2}, abi.E_ALIGN), ({"k_stride_head": 60}, abi.E_ALIGN), ({"v_stride_token": 12}, abi.E_ALIGN)])
+    ({"cu_k_addr": A + 2}, abi.E_ALIGN), ({"k_stride_head": 60}, abi.E_ALIGN), ({"v_stride_token": 12}, abi.E_ALIGN),
+    ({"k_stride_head": 0}, abi.E_SHAPE)])
 def test_prompt_attention_refusals(change, want):
     assert code("prompt_attention", prompt_arg(**change)) == want
 
@@ -121,7 +122,8 @@ def test_prompt_attention_refusals(change, want):
     ({"v_pages_addr": A + 2}, abi.E_ALIGN), ({"page_table_addr": 0}, abi.E_NULL_ARG),
     ({"context_lens_addr": A + 1}, abi.E_ALIGN), ({"mask_addr": A}, abi.E_SHAPE),
     ({"mask_addr": A + 1, "mask_words": 1}, abi.E_ALIGN), ({"k_page_stride_token": 100}, abi.E_ALIGN),
-    ({"v_page_stride_page": 4}, abi.E_ALIGN)])
+    ({"v_page_stride_page": 4}, abi.E_ALIGN), ({"v_page_stride_head": 0}, abi.E_SHAPE),
+    ({"k_page_stride_page": -2048}, abi.E_SHAPE)])
 def test_tree_attention_refusals(change, want):
     assert code("tree_attention", tree_arg(**change)) == want
 
