@@ -73,6 +73,66 @@ def test_rope_strided_views_and_in_place(dtype, interleaved):
     assert torch.equal(fused[:, :16], before[:, :16]) and torch.equal(fused[:, 528:], before[:, 528:])
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("hq,hk,d,rot", [(4, 2, 64, 64), (5, 0, 80, 48), (1, 1, 128, 32), (3, 2, 24, 16)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_of_many_tokens(dtype, hq, hk, d, rot, interleaved):
+    """Enough tokens for the whole-row form; rows of a wider buffer, one position outside the table."""
+    g = gen(hq * d)
+    t = 3700
+    fused = normal(g, (t, (hq + hk) * d + 16), dtype)
+    q, k = fused[:, :hq * d].view(t, hq, d), fused[:, hq * d:(hq + hk) * d].view(t, hk, d)
+    pos = torch.randint(0, 900, (t,), generator=g, dtype=torch.int32)
+    pos[1234] = 900
+    table = normal(g, (900, rot), F32)
+    dev = fused.cuda()
+    dq, dk = dev[:, :hq * d].view(t, hq, d), dev[:, hq * d:(hq + hk) * d].view(t, hk, d)
+    out_q, out_k = torch.full_like(dq, 3.0).contiguous(), torch.full_like(dk, 3.0).contiguous()
+    for inverse in (False, True):
+        ops.rope(dq, dk, pos.cuda(), table.cuda(), interleaved=interleaved, inverse=inverse, q_out=out_q, k_out=out_k)
+        assert took_bad_index()
+        on = pos < 900
+        for x, y in ((q, out_q), (k, out_k)):
+            want, bound = ref.rotate(x[on], pos[on], table, interleaved, inverse)
+            ref.assert_within(y.cpu()[on], want, bound)
+            assert (y[1234] == 3.0).all()
+    ops.rope(dq, dk, pos.cuda(), table.cuda(), interleaved=interleaved, q_out=dq, k_out=dk)
+    assert took_bad_index()
+    want, bound = ref.rotate(q[on], pos[on], table, interleaved)
+    ref.assert_within(dq.cpu()[on], want, bound)
+    assert torch.equal(dev[:, (hq + hk) * d:].cpu(), fused[:, (hq + hk) * d:])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads_first", [False, True])
+def test_rope_append_of_many_tokens(dtype, heads_first):
+    g = gen(91)
+    t, hq, hk, d, page = 3800, 3, 2, 64, 24
+    q, k, v = (normal(g, (t, h, d), dtype) for h in (hq, hk, hk))
+    pages = t // page + 5
+    shape = (pages, hk, page, d) if heads_first else (pages, page, hk, d)
+    kp, vp = (torch.full(shape, float("nan"), dtype=dtype, device="cuda") for _ in range(2))
+    if heads_first:
+        kp, vp = kp.transpose(1, 2), vp.transpose(1, 2)
+    slots = torch.randperm(pages * page, generator=g)[:t]
+    slots[7], slots[3000] = -1, pages * page
+    pos = torch.randint(0, 200, (t,), generator=g, dtype=torch.int32)
+    table = normal(g, (200, d), F32)
+    k_out = torch.empty(hk, t, d, dtype=dtype, device="cuda").transpose(0, 1)
+    out = ops.rope_append(q.cuda(), k.cuda(), v.cuda(), pos.cuda(), table.cuda(), slots.cuda(), kp, vp, k_out=k_out)
+    assert took_bad_index()
+    ref.assert_within(out, *ref.rotate(q, pos, table))
+    want, bound = ref.rotate(k, pos, table)
+    ref.assert_within(k_out, want, bound)
+    on = (slots >= 0) & (slots < pages * page)
+    kf, vf = kp.cpu().reshape(-1, hk, d), vp.cpu().reshape(-1, hk, d)
+    ref.assert_within(kf[slots[on]], want[on], bound[on])
+    assert torch.equal(vf[slots[on]], v[on])
+    rest = torch.ones(pages * page, dtype=torch.bool)
+    rest[slots[on]] = False
+    assert torch.isnan(kf[rest]).all() and torch.isnan(vf[rest]).all()
+
+
 def test_rope_unaligned_view_takes_the_elementwise_form():
     g = gen(6)
     buf = normal(g, (9 * 4 * 64 + 1,), F16).cuda()
