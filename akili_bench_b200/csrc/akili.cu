@@ -1237,7 +1237,7 @@ int entry_kb2(const Arg* a, const akili_ex_t* ex, akili_stream_t s) {
 // FFN hidden size, 11008 for 7B: 44 KB).
 constexpr size_t kMatvecSmemMax = 200 * 1024;
 
-// AKILI_PDL=0 launches the matrix-vector kernels without the programmatic
+// AKILI_PDL=0 launches the matrix-vector and serving kernels without the programmatic
 // dependent launch attribute (for A/B measurements).
 bool pdl_enabled() {
   static const bool on = [] {

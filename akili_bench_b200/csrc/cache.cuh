@@ -67,7 +67,9 @@ constexpr int kAcceptRows = 128;  // moves whose offsets are held at a time
 // entries are taken in ascending order by the thread that owns the column, so
 // moving in place needs no copy of the branch: a source is always read before
 // the entry whose destination it is, or in the same batch, whose loads all
-// come before its stores.
+// come before its stores.  Bound by its chain of latencies (lengths, indices,
+// pages, values): 16 sequences, 87 entries, 32 layers of 8 heads of 128 take
+// 5.5 us, 22 MB.
 template <typename U>
 __global__ void __launch_bounds__(kAcceptThreads) cache_accept_kernel(const AcceptArgs a) {
   griddep_wait();

@@ -26,6 +26,11 @@
 // per page part), 2 TMEM owner and MMA issuer, 3 loads the next item's Q, 4..7
 // softmax and output.  Q, S, P and O have two buffers each, so an item's first
 // scores are computed while the last one is still being written out.
+//
+// Measured: 32 contexts of 77 to 16383 tokens, one new token each, 32/8 heads
+// of 128, bf16: 174 us, 6.3 TB/s, 0.97 of the copy rate (the row form 242 us);
+// one context of 4001 tokens, 32 heads, fp16: 17 us from L2, 20 from HBM, of
+// which 10 are its 65 MB and the rest start, first loads and join.
 #pragma once
 #include "serving_attention.cuh"
 
@@ -163,7 +168,7 @@ __global__ void __launch_bounds__(kDcThreads, 1)
   griddep_launch_dependents();
   // Every warp finds the CTA's share by itself and the loaders look up their
   // first pages before the barrier: the first load leaves that much earlier
-  // (5500 -> XXXX cycles after the start).
+  // (5500 -> 4500 cycles after the start).
   SvWalk<N> walk;
   SvPiece pc;
   long long quota, total;

@@ -13,6 +13,13 @@
 // per share of its heads when there are few tokens); a thread keeps the
 // cosines and sines of its VEC pairs in registers and walks over the heads, so
 // the table is read once per token and thread, from L2.
+//
+// Measured: 8192 tokens, 32 + 8 heads of 128, fp16: 32 us, 5.3 TB/s (an
+// elementwise product of the same bytes: 27.5 us; the copy rate would be
+// 26.3).  Two heads a thread, persistent blocks with the next position read
+// ahead, and whole rows through shared memory by bulk copies measured 31 to
+// 36 us and more for the append; larger blocks less (256 threads 46 us).
+// 7 tokens: 2.2 us.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
