@@ -207,9 +207,9 @@ DEFAULT_REFERENCE_ROOT = "/root/reference"
 
 def reference_root(arg: str | None = None) -> str | None:
     """The reference tree: the argument, else $AKILI_REFERENCE_ROOT, else
-    DEFAULT_REFERENCE_ROOT; None when that is not a directory."""
+    DEFAULT_REFERENCE_ROOT; None when that holds no benchmarks."""
     ref = arg or os.environ.get("AKILI_REFERENCE_ROOT") or DEFAULT_REFERENCE_ROOT
-    return ref if os.path.isdir(ref) else None
+    return ref if os.path.isdir(os.path.join(ref, "benchmarks")) else None
 
 
 def main() -> int:
