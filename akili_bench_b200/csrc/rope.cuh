@@ -14,11 +14,12 @@
 // cosines and sines of its VEC pairs in registers and walks over the heads, so
 // the table is read once per token and thread, from L2.
 //
-// Measured: 8192 tokens, 32 + 8 heads of 128, fp16: 32 us, 5.3 TB/s (an
+// Measured: 8192 tokens, 32 + 8 heads of 128, fp16: 30 us, 5.7 TB/s (an
 // elementwise product of the same bytes: 27.5 us; the copy rate would be
-// 26.3).  Two heads a thread, persistent blocks with the next position read
-// ahead, and whole rows through shared memory by bulk copies measured 31 to
-// 36 us and more for the append; larger blocks less (256 threads 46 us).
+// 26.3).  Blocks of 128 threads measured 32 us (24 against 22 for the append),
+// of 256 threads 46, of one warp 31 (and 16 against 11 for 2049 tokens in fp32);
+// two heads a thread, persistent blocks with the next position read ahead, and
+// whole rows through shared memory by bulk copies 31 to 36 us.
 // 7 tokens: 2.2 us.
 #pragma once
 #include <cuda_bf16.h>
@@ -30,7 +31,7 @@
 
 namespace akili {
 
-constexpr int kRopeThreads = 128;
+constexpr int kRopeThreads = 64;
 
 __device__ __forceinline__ void record_bad_index() { atomicCAS(&g_status, 0u, AKILI_STATUS_BAD_INDEX); }
 

@@ -115,7 +115,7 @@ int run_rope(const akili_rope_arg_t* a, bool append, cudaStream_t st) {
     for (int i = 0; i < 3; ++i) { r.ko_st[i] = a->k_page_stride[i]; r.vo_st[i] = a->v_page_stride[i]; }
   // 16-byte accesses where every vector of every head starts on 16 bytes
   const int64_t n = 16 / es;
-  bool vec = a->table_addr % 16 == 0 && (a->rot_dim / 2) % n == 0 && (a->head_dim - a->rot_dim) % n == 0 && a->head_dim / (2 * n) <= kRopeThreads;
+  bool vec = a->table_addr % 16 == 0 && (a->rot_dim / 2) % n == 0 && (a->head_dim - a->rot_dim) % n == 0;
   if (a->q_heads)
     vec = vec && (a->q_addr | a->q_out_addr) % 16 == 0 && all_multiples(a->q_stride, n) &&
           all_multiples(a->q_out_stride, n);

@@ -43,7 +43,7 @@ def took_bad_index():
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 @pytest.mark.parametrize("tokens,hq,hk,d,rot", [(1, 1, 1, 8, 8), (5, 4, 2, 64, 64), (33, 7, 1, 96, 64), (2, 32, 8, 128, 128),
                                                (300, 3, 3, 80, 20), (3, 2, 0, 10, 6), (4, 0, 5, 256, 32),
-                                               (700, 32, 8, 128, 128)])
+                                               (700, 32, 8, 128, 128), (3, 2, 1, 1040, 640)])
 @pytest.mark.parametrize("interleaved,inverse", [(False, False), (True, False), (False, True), (True, True)])
 def test_rope(dtype, tokens, hq, hk, d, rot, interleaved, inverse):
     g = gen(tokens * 131 + d)
@@ -296,6 +296,7 @@ PROMPTS = [
     ([700, 513], None, 2, 1, 128),
     ([31, 65], [1000, 65], 16, 2, 120),
     ([1, 2], None, 72, 1, 64),
+    ([5, 70], None, 131, 1, 64),           # a group that no divisor packs
 ]
 
 
@@ -480,6 +481,7 @@ TREES = [
     ([4000, 17], [40, 64], 256, 8, 1, 128, False, True),
     ([90], [300], 40, 2, 1, 128, False, True),
     ([1500] * 3, [1] * 3, 16, 64, 1, 128, False, False),
+    ([300, 9], [1, 2], 16, 131, 1, 64, False, False),
 ]
 
 
@@ -591,6 +593,22 @@ def test_tree_attention_layers_view_workspace_and_repeat():
         o, _, bound, _ = ref.attend(q[at:at + m].cpu(), ks[b], vs[b], ref.causal(m, c + m))
         ref.assert_within(first[at:at + m], o, bound)
         at += m
+
+
+def test_tree_attention_workspace_must_be_large_enough():
+    g = gen(26)
+    kp, vp, table, _, _ = make_cache(g, [40], 8, 1, 64, F16)
+    q = normal(g, (1, 2, 64), F16).cuda()
+    args = (q, kp, vp, table.cuda(), i32([39]).cuda(), i32([0, 1]).cuda())
+    n = ops.tree_attention_workspace(q, kp, args[3], args[4])
+    for size, code in ((n - 1, abi.E_WORKSPACE), (n, abi.OK)):
+        ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+        if code == abi.OK:
+            ops.tree_attention(*args, workspace=ws)
+        else:
+            with pytest.raises(abi.AkiliError) as e:
+                ops.tree_attention(*args, workspace=ws)
+            assert e.value.code == code
 
 
 def test_tree_attention_invalid_pages_read_as_zeros():
