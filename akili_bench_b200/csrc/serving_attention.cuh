@@ -70,10 +70,10 @@ constexpr int kSvRows = 128;  // rows of a tile
 constexpr int kSvKeys = 128;  // keys of a block
 constexpr int kSvThreads = 640;
 constexpr int kSvJoinThreads = 256;
-// Blocks that share a cut item: the rows of the few-row form, the columns of
-// the row forms.
-template <int kTileRows>
-constexpr int kSvJoinSplit = kTileRows < kSvRows ? (kTileRows + 7) / 8 : kTileRows / 32;
+// Blocks that share a cut item: the rows of the few-row form (8 a block), the
+// columns of the row forms (a thread takes 16 of a row).
+template <int kTileRows, int DP>
+constexpr int kSvJoinSplit = kTileRows < kSvRows ? (kTileRows + 7) / 8 : DP / 16 * kTileRows / kSvJoinThreads;
 
 struct ServingArgs {
   const void* q;
@@ -85,6 +85,7 @@ struct ServingArgs {
   const int* page_table;
   const unsigned int* mask;
   float* parts;  // paged keys: O, m and l of cut items
+  int4* cuts;    // row forms, paged keys: the cut item that starts in each share
   int q_heads, kv_heads, group, head_dim, batch, total_q, total_k, causal;
   int pack;         // heads of a token in one tile; the head groups are q_heads / pack
   int head_groups;  // q_heads / pack
@@ -574,9 +575,10 @@ __global__ void __maxnreg__(96)
   SvPromptLine<kPair> line;
   SvWalk<kTileRows> walk;
   bool more = true;
+  [[maybe_unused]] long long quota = 1;
   if (warp == 19) {
     if constexpr (kPaged) {
-      long long quota, total;
+      long long total;
       more = sv_share<kTileRows>(a, blockIdx.x, gridDim.x, walk, &quota, &total);
     } else {
       line.load(a);
@@ -609,10 +611,19 @@ __global__ void __maxnreg__(96)
     uint32_t q_used[2] = {0, 0};   // loads of each Q tile
     uint32_t asked = 0;            // requests for further blocks
     uint32_t id = blockIdx.x;
+    if constexpr (kPaged)
+      if (lane == 0) a.cuts[2 * blockIdx.x].x = 0;
     while (ok) {
       SvPiece p;
       if constexpr (kPaged) {
         more = more && walk.next(a, blockIdx.x, p);
+        if (more && p.part >= 0 && p.kb == 0 && lane == 0) {
+          // starts here and is cut by the end of the share: for the join
+          const long long last = (p.first + walk.blocks - 1) / quota;
+          a.cuts[2 * blockIdx.x] = make_int4(static_cast<int>(last) - static_cast<int>(blockIdx.x) + 1, p.part, p.s.n,
+                                             p.tile * (kTileRows / kSvRows) * a.tile_tokens);
+          a.cuts[2 * blockIdx.x + 1] = make_int4(p.s.q0, p.hk, 0, 0);
+        }
       } else {
         if (count > 0) {
           // the block that was asked for when the last piece was handed out
@@ -1199,11 +1210,10 @@ __global__ void __maxnreg__(96)
 // Adds up the parts of the item that starts in share c = blockIdx.x and goes
 // on past its end, in order.
 //   m = max m_p,  o = sum 2^(m_p - m) O_p / sum 2^(m_p - m) l_p
-// Row forms: a thread per (row, four columns), rows along the lanes, as the
-// parts are laid out.  Few-row form (parts row by row): a warp per row.
+// Few-row form, whose parts lie row by row: a warp per row.  (Its blocks find
+// their cut item while the parts are still being computed.)
 template <int DP, typename T, int kTileRows>
 __global__ void __launch_bounds__(kSvJoinThreads) attention_join_kernel(const __grid_constant__ ServingArgs a) {
-  constexpr bool kByRow = kTileRows < kSvRows;
   __shared__ int from, parts, slot0, first, tokens, q0, hk;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
@@ -1220,7 +1230,7 @@ __global__ void __launch_bounds__(kSvJoinThreads) attention_join_kernel(const __
         from = blockIdx.x;
         parts = static_cast<int>(last) - blockIdx.x + 1;
         slot0 = p.part;
-        first = kByRow ? p.tile * kTileRows : p.tile * (kTileRows / kSvRows) * a.tile_tokens;
+        first = p.tile * kTileRows;
         tokens = p.s.n;
         q0 = p.s.q0;
         hk = p.hk;
@@ -1236,24 +1246,17 @@ __global__ void __launch_bounds__(kSvJoinThreads) attention_join_kernel(const __
   constexpr size_t kM = static_cast<size_t>(kTileRows) * DP, kL = static_cast<size_t>(kTileRows) * (DP + 1);
   // row r of the item -> its token and head within the group; false if it is nobody's
   auto row_of = [&](int r, int* tok, int* head) {
-    if constexpr (kByRow) {
-      const int row = first + r;
-      *tok = row / a.group;
-      *head = row - *tok * a.group;
-      return *tok < tokens;
-    } else {
-      const int in = r % kSvRows, t = in / a.pack;
-      *tok = first + r / kSvRows * a.tile_tokens + t;
-      *head = in - t * a.pack;
-      return t < a.tile_tokens && *tok < tokens;
-    }
+    const int row = first + r;
+    *tok = row / a.group;
+    *head = row - *tok * a.group;
+    return *tok < tokens;
   };
   // Eight parts at a time, all of whose loads are under way together.
   auto join_row = [&](int r, int unit0, int unit_step) {
     int tok, head;
     if (!row_of(r, &tok, &head)) return;
     const long long qrow = q0 + tok;
-    const int qh = hk * (kByRow ? a.group : a.pack) + head;
+    const int qh = hk * a.group + head;
     for (int unit = unit0; unit * 4 < a.head_dim; unit += unit_step) {
       float o[4] = {}, m = -INFINITY, l = 0.0f;
       for (int i0 = 0; i0 < parts; i0 += 8) {
@@ -1265,8 +1268,7 @@ __global__ void __launch_bounds__(kSvJoinThreads) attention_join_kernel(const __
           const float* p = part(on ? i0 + i : i0);
           pm[i] = on ? p[kM + r] : -INFINITY;
           pl[i] = p[kL + r];
-          pv[i] = *reinterpret_cast<const float4*>(
-              p + (kByRow ? static_cast<size_t>(r) * DP + unit * 4 : (static_cast<size_t>(unit) * kTileRows + r) * 4));
+          pv[i] = *reinterpret_cast<const float4*>(p + static_cast<size_t>(r) * DP + unit * 4);
         }
         float top = m;
 #pragma unroll
@@ -1297,13 +1299,91 @@ __global__ void __launch_bounds__(kSvJoinThreads) attention_join_kernel(const __
       if (a.lse != nullptr && unit == 0) a.lse[qrow * a.q_heads + qh] = (m + log2f(l)) * 0.6931471805599453f;
     }
   };
-  if constexpr (kByRow) {
-    for (int r = blockIdx.y * (kSvJoinThreads / 32) + warp; r < kTileRows; r += gridDim.y * (kSvJoinThreads / 32))
-      join_row(r, lane, 32);
-  } else {
-    constexpr int kPer = kSvJoinThreads / kTileRows;  // threads of a row within a block
-    join_row(threadIdx.x % kTileRows, blockIdx.y * kPer + threadIdx.x / kTileRows, gridDim.y * kPer);
-  }
+  for (int r = blockIdx.y * (kSvJoinThreads / 32) + warp; r < kTileRows; r += gridDim.y * (kSvJoinThreads / 32))
+    join_row(r, lane, 32);
+}
+
+// The same for the row forms, whose parts lie by four columns, rows along the
+// lanes: a thread per (row, 16 columns).  No register of an SM is free for
+// these blocks before its CTA of the attention ends, so they do not look for
+// their item but read it from `cuts`.  Nearly all items are cut once or twice:
+// the loads of two parts (or of four, half the columns at a time) are under
+// way together.
+template <int DP, typename T, int kTileRows>
+__global__ void __launch_bounds__(kSvJoinThreads) attention_join_rows_kernel(const __grid_constant__ ServingArgs a) {
+  griddep_wait();  // the parts
+  griddep_launch_dependents();
+  const int4 cut = a.cuts[2 * blockIdx.x];
+  const int parts = cut.x;
+  if (parts == 0) return;
+  const int4 seq = a.cuts[2 * blockIdx.x + 1];
+  constexpr size_t kSlot = static_cast<size_t>(kTileRows) * (DP + 2);
+  constexpr size_t kM = static_cast<size_t>(kTileRows) * DP, kL = static_cast<size_t>(kTileRows) * (DP + 1);
+  constexpr int kPer = kSvJoinThreads / kTileRows;  // threads of a row within a block
+  const int r = threadIdx.x % kTileRows;
+  const int c0 = (blockIdx.y * kPer + threadIdx.x / kTileRows) * 16;
+  const int in = r % kSvRows, t = in / a.pack;
+  const int tok = cut.w + r / kSvRows * a.tile_tokens + t;
+  if (t >= a.tile_tokens || tok >= cut.z || c0 >= a.head_dim) return;
+  const long long qrow = seq.x + tok;
+  const int qh = seq.y * a.pack + in - t * a.pack;
+  auto part = [&](int i) { return a.parts + (i == 0 ? cut.y : 2 * (static_cast<int>(blockIdx.x) + i)) * kSlot; };
+  T* out = static_cast<T*>(a.o) + qrow * a.o_st[0] + qh * a.o_st[1];
+  float m = -INFINITY;
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) m = fmaxf(m, part(i)[kM + r]);
+  const float sub = m == -INFINITY ? 0.0f : m;
+  // kBatch parts and 8 / kBatch units of four columns at a time
+  auto join = [&](auto batch) {
+    constexpr int kBatch = decltype(batch)::value, kUnits = 8 / kBatch;
+#pragma unroll 1
+    for (int c = c0; c < c0 + 16 && c < a.head_dim; c += 4 * kUnits) {
+      float o[4 * kUnits] = {}, l = 0.0f;
+#pragma unroll 1
+      for (int i0 = 0; i0 < parts; i0 += kBatch) {
+        float pm[kBatch], pl[kBatch];
+        float4 pv[kBatch][kUnits];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const bool on = i0 + i < parts;
+          const float* p = part(on ? i0 + i : i0);
+          pm[i] = on ? p[kM + r] : -INFINITY;
+          pl[i] = p[kL + r];
+#pragma unroll
+          for (int u = 0; u < kUnits; ++u)
+            pv[i][u] = *reinterpret_cast<const float4*>(p + (static_cast<size_t>(c / 4 + u) * kTileRows + r) * 4);
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const float w = exp2f(pm[i] - sub);
+          if (w != 0.0f) {  // (a part that saw nothing of the row holds anything)
+            l += w * pl[i];
+#pragma unroll
+            for (int u = 0; u < kUnits; ++u) {
+              o[4 * u] += w * pv[i][u].x;
+              o[4 * u + 1] += w * pv[i][u].y;
+              o[4 * u + 2] += w * pv[i][u].z;
+              o[4 * u + 3] += w * pv[i][u].w;
+            }
+          }
+        }
+      }
+      const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+      for (int u = 0; u < kUnits; u += 2) {
+        if (c + 4 * u >= a.head_dim) continue;
+        uint4 v;
+        v.x = pack2<T>(o[4 * u] * inv, o[4 * u + 1] * inv);
+        v.y = pack2<T>(o[4 * u + 2] * inv, o[4 * u + 3] * inv);
+        v.z = pack2<T>(o[4 * u + 4] * inv, o[4 * u + 5] * inv);
+        v.w = pack2<T>(o[4 * u + 6] * inv, o[4 * u + 7] * inv);
+        *reinterpret_cast<uint4*>(out + c + 4 * u) = v;
+      }
+      if (a.lse != nullptr && c == 0) a.lse[qrow * a.q_heads + qh] = (m + log2f(l)) * 0.6931471805599453f;
+    }
+  };
+  if (parts == 2) join(std::integral_constant<int, 2>{});
+  else join(std::integral_constant<int, 4>{});
 }
 
 }  // namespace akili

@@ -386,9 +386,11 @@ int launch_cache(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap
     rc = launch_dependent(kern, dim3(blocks), kDcThreads, smem, st, tk, tv, g);
   }
   if (rc) return rc;
-  // (its blocks find their cut item while the parts are still being computed)
-  return launch_dependent(attention_join_kernel<DP, T, kTileRows>, dim3(blocks, kSvJoinSplit<kTileRows>),
-                          kSvJoinThreads, 0, st, g);
+  const dim3 join(blocks, kSvJoinSplit<kTileRows, DP>);
+  if constexpr (kTileRows >= kSvRows)
+    return launch_dependent(attention_join_rows_kernel<DP, T, kTileRows>, join, kSvJoinThreads, 0, st, g);
+  else
+    return launch_dependent(attention_join_kernel<DP, T, kTileRows>, join, kSvJoinThreads, 0, st, g);
 }
 
 template <int DP, typename T>
@@ -481,9 +483,13 @@ int tree_tile_rows(const akili_tree_attention_arg_t* a) {
   return form;
 }
 
-// Two parts (O, m, l) for each share of the line of key blocks.
-size_t tree_workspace_bytes(const DevInfo& di, const akili_tree_attention_arg_t* a) {
+// Two parts (O, m, l) for each share of the line of key blocks, then (row
+// forms) what the join has to know of each share.
+size_t tree_parts_bytes(const DevInfo& di, const akili_tree_attention_arg_t* a) {
   return 2ull * di.sms * tree_tile_rows(a) * ((a->head_dim <= 64 ? 64 : 128) + 2) * sizeof(float);
+}
+size_t tree_workspace_bytes(const DevInfo& di, const akili_tree_attention_arg_t* a) {
+  return tree_parts_bytes(di, a) + (tree_tile_rows(a) >= kSvRows ? 2 * di.sms * sizeof(int4) : 0);
 }
 
 int run_tree_attention(const akili_tree_attention_arg_t* a, cudaStream_t st) {
@@ -516,6 +522,7 @@ int run_tree_attention(const akili_tree_attention_arg_t* a, cudaStream_t st) {
   g.page_table = static_cast<const int*>(P(a->page_table_addr));
   g.mask = static_cast<const unsigned int*>(P(a->mask_addr));
   g.parts = reinterpret_cast<float*>(parts);
+  g.cuts = reinterpret_cast<int4*>(parts + tree_parts_bytes(di, a));
   g.q_heads = a->q_heads; g.kv_heads = a->kv_heads; g.group = static_cast<int>(a->q_heads / a->kv_heads);
   g.head_dim = a->head_dim; g.batch = a->batch; g.total_q = a->total_q;
   g.num_pages = a->num_pages; g.page_size = a->page_size; g.max_pages = a->max_pages; g.mask_words = a->mask_words;
