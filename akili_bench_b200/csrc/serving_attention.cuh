@@ -1195,7 +1195,8 @@ __global__ void __maxnreg__(96)
           }
         }
       }
-      tc_fence_before();  // O has been read before the next P is announced
+      tc_fence_before();  // O has been read before the next P is announced,
+      if constexpr (!kPair) named_bar_sync(quad_bar, 128);  // by the other stream's warps too
       drop_task();
     }
   }
