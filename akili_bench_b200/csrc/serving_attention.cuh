@@ -47,7 +47,7 @@
 // (sequence, head group, tile) items form one line that is cut into equal
 // shares, one per CTA, so uneven lengths and few long sequences fill the GPU
 // alike; an item that is cut leaves its parts (O, m, l in fp32) in the
-// workspace and attention_join_kernel adds them up in order.
+// workspace and a join kernel adds them up in order.
 //
 // Bound by the chain of a block: scores, TMEM load, maximum, exponentials, P,
 // product.  One stream alone would take 2300 cycles a block; the two overlap to
@@ -55,7 +55,7 @@
 // the time is the same).  Measured: 8 causal prompts of 4096 tokens, 32 heads
 // of 128, fp16: 1.21 ms, 907 TFLOP/s of visible pairs; six uneven bf16 prompts
 // with 32/8 heads: 960 TFLOP/s; 24 short ones with 14/2 heads of 64: 12 us; 16
-// drafted trees over 700 to 5999 tokens: 80 us.
+// drafted trees over 700 to 5999 tokens: 73 us (79 with nothing in L2).
 #pragma once
 #include <type_traits>
 
@@ -1309,7 +1309,8 @@ __global__ void __launch_bounds__(kSvJoinThreads) attention_join_kernel(const __
 // these blocks before its CTA of the attention ends, so they do not look for
 // their item but read it from `cuts`.  Nearly all items are cut once or twice:
 // the loads of two parts (or of four, half the columns at a time) are under
-// way together.
+// way together.  The join of 16 drafted trees (275 parts of up to 133 KB) takes
+// 10.8 us alone; eight parts at a time, four columns a thread, took 21.
 template <int DP, typename T, int kTileRows>
 __global__ void __launch_bounds__(kSvJoinThreads) attention_join_rows_kernel(const __grid_constant__ ServingArgs a) {
   griddep_wait();  // the parts
