@@ -54,7 +54,7 @@
 // 60% of the tensor pipe (and of the exponential unit; without exponentials
 // the time is the same).  Measured: 8 causal prompts of 4096 tokens, 32 heads
 // of 128, fp16: 1.21 ms, 907 TFLOP/s of visible pairs; six uneven bf16 prompts
-// with 32/8 heads: 960 TFLOP/s; 24 short ones with 14/2 heads of 64: 12 us; 16
+// with 32/8 heads: 945 TFLOP/s; 24 short ones with 14/2 heads of 64: 12 us; 16
 // drafted trees over 700 to 5999 tokens: 73 us (79 with nothing in L2).
 #pragma once
 #include <type_traits>
