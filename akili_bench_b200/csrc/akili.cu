@@ -1204,18 +1204,35 @@ int entry(const Arg* a, const akili_ex_t* ex, akili_stream_t s) {
 }
 
 static_assert((0x1000u | kSiteSelfTest) == AKILI_STATUS_SELFTEST, "status code of the self-test wait");
+static_assert((0x1000u | kSiteSelfTestShared) == AKILI_STATUS_SELFTEST_SHARED, "status code of the shared wait");
 
-// One CTA waits on an mbarrier that nothing arrives at, bounded by limit_ns:
-// the wait gives up, records kSiteSelfTest and the kernel returns.
+// One CTA whose waits give up: a wait on an mbarrier that nothing arrives at,
+// bounded by limit_ns, records kSiteSelfTest (warp 0).  Two warps that decide
+// together (mbar_wait_together) wait for a phase that completes after the limit of
+// the one and before that of the other; should they not end alike, the status
+// becomes kSiteSelfTestShared (warps 1 and 2; warp 3 completes the phase).
 __global__ void selftest_wait_kernel(uint64_t limit_ns) {
-  __shared__ alignas(8) uint64_t bar;
+  __shared__ alignas(8) uint64_t bar, late;
+  __shared__ bool went_on[2];
+  const uint32_t warp = warp_id(), lane = lane_id();
   if (threadIdx.x == 0) {
     mbar_init(&bar, 1);
+    mbar_init(&late, 1);
     fence_mbar_init();
   }
   __syncthreads();
-  if (threadIdx.x == 0) mbar_wait_for(&bar, 0, kSiteSelfTest, limit_ns);
+  if (warp == 0) {
+    if (lane == 0) mbar_wait_for(&bar, 0, kSiteSelfTest, limit_ns);
+  } else if (warp < 3) {
+    const bool on = mbar_wait_together<64>(&late, 0, kSiteSelfTest, 1, warp == 1 ? limit_ns : 8 * limit_ns);
+    if (lane == 0) went_on[warp - 1] = on;
+  } else if (lane == 0) {
+    const uint64_t t0 = globaltimer();
+    while (globaltimer() - t0 < 2 * limit_ns) __nanosleep(1000);
+    mbar_arrive(&late);
+  }
   __syncthreads();
+  if (threadIdx.x == 0 && (went_on[0] || went_on[1])) atomicExch(&g_status, 0x1000u | kSiteSelfTestShared);
 }
 
 // kb2_* entries: fp32 in, fp32 out; an akili_ex_t may only add a workspace.
@@ -1964,7 +1981,7 @@ int akili_selftest_wait_timeout(uint32_t limit_us, akili_stream_t s) {
   DevInfo di;
   int rc = device_info(&di);
   if (rc) return rc;
-  selftest_wait_kernel<<<1, 32, 0, S(s)>>>(uint64_t(limit_us) * 1000ull);
+  selftest_wait_kernel<<<1, 128, 0, S(s)>>>(uint64_t(limit_us) * 1000ull);
   return launch_status();
 }
 

@@ -495,21 +495,6 @@ __device__ __forceinline__ uint64_t mask_window(const unsigned int* row, int wor
   return v;
 }
 
-// Barrier of kThreads threads that returns whether any of them votes.
-template <int kThreads>
-__device__ __forceinline__ bool vote_barrier(uint32_t id, bool vote) {
-  uint32_t any;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, %2, %3, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(any)
-      : "r"(static_cast<uint32_t>(vote)), "r"(id), "n"(kThreads)
-      : "memory");
-  return any != 0;
-}
-
 // ----------------------------------------------------------------- kernel --
 template <int DP, typename T, bool kPaged, bool kPair>
 __global__ void __maxnreg__(96)
@@ -589,10 +574,11 @@ __global__ void __maxnreg__(96)
   const uint32_t tmem = ctl->tmem;
 
   uint32_t n_task = 0;  // pieces taken so far
+  auto wait_task = [&](uint64_t* full, uint32_t parity) { return mbar_wait(full, parity, kSiteProducerEmpty); };
   // The next piece for a worker warp; nullptr: no more work, or a wait gave up (*ok false).
-  auto take_task = [&](bool* ok) -> const SvTask* {
+  auto take_task = [&](bool* ok, auto wait) -> const SvTask* {
     const uint32_t slot = n_task % kSvTasks;
-    *ok = __all_sync(0xffffffffu, mbar_wait(&ctl->task_full[slot], (n_task / kSvTasks) & 1, kSiteProducerEmpty));
+    *ok = __all_sync(0xffffffffu, wait(&ctl->task_full[slot], (n_task / kSvTasks) & 1));
     const SvTask* t = &ctl->task[slot];
     if (!*ok || t->loads < 0) return nullptr;
     ++n_task;
@@ -732,7 +718,7 @@ __global__ void __maxnreg__(96)
     int st = 0;
     uint32_t round = 0, issued = 0;
     bool ok = true;
-    while (const SvTask* t = take_task(&ok)) {
+    while (const SvTask* t = take_task(&ok, wait_task)) {
       const int loads = t->loads, kb = t->kb, m = t->m, k0 = t->k0, b = t->b;
       const int kv_head = t->hk / a.groups_per_kv;
       drop_task();
@@ -852,7 +838,7 @@ __global__ void __maxnreg__(96)
       }
       umma_commit_warp(&ctl->s_full[t]);
     };
-    while (const SvTask* task = take_task(&ok)) {
+    while (const SvTask* task = take_task(&ok, wait_task)) {
       const int loads = task->loads, n0 = task->blocks[0], n1 = task->blocks[1];
       const int tail = task->m - task->kb * kSvKeys;  // keys from this piece's first block on
       drop_task();
@@ -937,8 +923,13 @@ __global__ void __maxnreg__(96)
     auto swap_slot = [&](uint32_t ev) {
       return xchg + ((L::kXBufs == 2 ? (ev & 1) * 2 : 0) + grp) * (2 * kSvRows);
     };
+    // (the warps that meet at barriers go on or end together)
+    auto wait_task_together = [&](uint64_t* full, uint32_t parity) {
+      return mbar_wait_together<kPair ? 64 : 128>(full, parity, kSiteProducerEmpty, kPair ? pair_bar : quad_bar,
+                                                  kWaitTimeoutNs);
+    };
     bool ok = true;
-    while (const SvTask* task = take_task(&ok)) {
+    while (const SvTask* task = take_task(&ok, wait_task_together)) {
       const uint32_t piece_parity = n_task & 1;
       // ---- this piece's row
       const int tok = task->tok0 + (kPair ? grp * a.tile_tokens : 0) + row_tok;

@@ -38,6 +38,7 @@ enum WaitSite : uint32_t {
   kSiteSelfTest = 12,
   kSiteExchange = 13,
   kSiteRowSync = 14,
+  kSiteSelfTestShared = 15,
 };
 
 __device__ __forceinline__ uint64_t globaltimer() {
@@ -215,6 +216,31 @@ __device__ __forceinline__ void fence_async_shared() {
 }
 __device__ __forceinline__ void named_bar_sync(uint32_t id, uint32_t nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
+}
+
+// Barrier of kThreads threads that returns whether any of them votes.
+template <int kThreads>
+__device__ __forceinline__ bool vote_barrier(uint32_t id, bool vote) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, %2, %3, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(static_cast<uint32_t>(vote)), "r"(id), "n"(kThreads)
+      : "memory");
+  return any != 0;
+}
+
+// A bounded wait that ends alike for kThreads threads, which all call it with
+// the same barrier id: false for all of them if any gave up.  (A warp that
+// went on without the others would wait for them at their next barrier, which
+// has no limit.)
+template <int kThreads>
+__device__ __forceinline__ bool mbar_wait_together(uint64_t* bar, uint32_t parity, uint32_t site, uint32_t id,
+                                                   uint64_t limit_ns) {
+  return !vote_barrier<kThreads>(id, !mbar_wait_for(bar, parity, site, limit_ns));
 }
 
 // ---------------------------------------------------------------- tcgen05 --

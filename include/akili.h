@@ -471,9 +471,13 @@ int akili_device_status(uint32_t* status, int clear);
 /* Self-test of device-side failure detection: launches one CTA that waits
  * on an mbarrier nothing arrives at, with a limit of `limit_us` microseconds
  * (1..1000000).  The wait gives up, records AKILI_STATUS_SELFTEST in the
- * status word and the kernel returns; the context stays usable.  Returns
- * AKILI_OK once launched; read the outcome with akili_device_status(). */
+ * status word and the kernel returns; the context stays usable.  Two warps
+ * that decide together whether to go on also wait for a phase that completes
+ * after the limit of only one of them: both have to give up, else the status
+ * is AKILI_STATUS_SELFTEST_SHARED.  Returns AKILI_OK once launched; read the
+ * outcome with akili_device_status(). */
 #define AKILI_STATUS_SELFTEST 0x100Cu
+#define AKILI_STATUS_SELFTEST_SHARED 0x100Fu
 int akili_selftest_wait_timeout(uint32_t limit_us, akili_stream_t stream);
 
 /* Number of kernel launches this library has issued in this process
