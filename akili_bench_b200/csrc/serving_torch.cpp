@@ -12,10 +12,13 @@
 
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Stream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <initializer_list>
+#include <optional>
 #include <string>
 
 #include "../../include/akili_serving.h"
@@ -126,23 +129,54 @@ uint64_t index(const at::Tensor& t, const at::Tensor& first, std::initializer_li
   return addr(t);
 }
 
-akili_stream_t stream_of(PyObject* o) {
-  if (o == Py_None) return reinterpret_cast<akili_stream_t>(c10::cuda::getCurrentCUDAStream().stream());
-  PyObject* h = PyObject_GetAttrString(o, "cuda_stream");
-  if (!h) throw PyError{};
-  void* p = PyLong_AsVoidPtr(h);
-  Py_DECREF(h);
-  if (!p && PyErr_Occurred()) throw PyError{};
-  return static_cast<akili_stream_t>(p);
-}
+// The stream of a call.  What the call allocates comes from that stream's
+// memory: a block that the allocator takes back from the caller's current
+// stream may still be read or written by what is queued there, which this
+// stream does not wait for.  The caller goes on to use the result on its own
+// stream, which the allocator is told.
+class CallStream {
+ public:
+  explicit CallStream(PyObject* o) : caller_(c10::cuda::getCurrentCUDAStream()), handle_(caller_.stream()) {
+    if (o == Py_None) return;
+    const c10::cuda::CUDAStream s = given(o, caller_.device_index());
+    handle_ = s.stream();
+    if (handle_ != caller_.stream()) guard_.emplace(s);
+  }
+  akili_stream_t handle() const { return reinterpret_cast<akili_stream_t>(handle_); }
+  at::Tensor empty(at::IntArrayRef sizes, const at::TensorOptions& options) const {
+    at::Tensor t = at::empty(sizes, options);
+    if (guard_) t.record_stream(caller_);
+    return t;
+  }
+
+ private:
+  static c10::cuda::CUDAStream given(PyObject* o, c10::DeviceIndex device) {
+    if (THPStream_Check(o)) {
+      const auto* s = reinterpret_cast<const THPStream*>(o);
+      if (s->device_type != static_cast<int64_t>(c10::DeviceType::CUDA) || s->device_index != device)
+        fail(PyExc_ValueError, "stream must be a CUDA stream of the current device");
+      return c10::cuda::CUDAStream::unpack3(s->stream_id, device, c10::DeviceType::CUDA);
+    }
+    PyObject* h = PyObject_GetAttrString(o, "cuda_stream");
+    if (!h) throw PyError{};
+    void* p = PyLong_AsVoidPtr(h);
+    Py_DECREF(h);
+    if (!p && PyErr_Occurred()) throw PyError{};
+    return c10::cuda::getStreamFromExternal(static_cast<cudaStream_t>(p), device);
+  }
+
+  c10::cuda::CUDAStream caller_;
+  cudaStream_t handle_;
+  std::optional<c10::cuda::CUDAStreamGuard> guard_;
+};
 
 template <size_t n>
 void strides(int64_t (&to)[n], const at::Tensor& t, int64_t from = 0) {
   for (size_t i = 0; i < n; ++i) to[i] = t.stride(from + static_cast<int64_t>(i));
 }
 
-at::Tensor given_or_like(PyObject* o, const at::Tensor& like, const char* name) {
-  if (o == Py_None) return at::empty(like.sizes(), like.options());
+at::Tensor given_or_like(PyObject* o, const at::Tensor& like, const char* name, const CallStream& st) {
+  if (o == Py_None) return st.empty(like.sizes(), like.options());
   const at::Tensor& t = tensor(o, name);
   values(like, t, name);
   if (t.sizes() != like.sizes())
@@ -180,12 +214,13 @@ PyObject* rope(PyObject* const* v) {
   akili_rope_arg_t a = {};
   const at::Tensor &q = tensor(v[0], "q"), &k = tensor(v[1], "k");
   rope_common(a, q, k, tensor(v[2], "positions"), tensor(v[3], "table"), truth(v[4]), truth(v[5]));
-  const at::Tensor q_out = given_or_like(v[6], q, "q_out"), k_out = given_or_like(v[7], k, "k_out");
+  const CallStream st(v[8]);
+  const at::Tensor q_out = given_or_like(v[6], q, "q_out", st), k_out = given_or_like(v[7], k, "k_out", st);
   a.q_out_addr = addr(q_out);
   a.k_out_addr = addr(k_out);
   strides(a.q_out_stride, q_out);
   strides(a.k_out_stride, k_out);
-  if (const int rc = akili_rope(&a, stream_of(v[8]))) refuse("rope", rc);
+  if (const int rc = akili_rope(&a, st.handle())) refuse("rope", rc);
   return Py_BuildValue("(NN)", THPVariable_Wrap(q_out), THPVariable_Wrap(k_out));
 }
 
@@ -202,7 +237,8 @@ PyObject* rope_append(PyObject* const* v) {
   shape_is(kp, {-1, -1, k.size(1), k.size(2)}, "k_pages");
   shape_is(vp, {kp.size(0), kp.size(1), k.size(1), k.size(2)}, "v_pages");
   a.slots_addr = index(tensor(v[5], "slots"), q, {q.size(0)}, "slots", at::kLong);
-  const at::Tensor q_out = given_or_like(v[9], q, "q_out");
+  const CallStream st(v[11]);
+  const at::Tensor q_out = given_or_like(v[9], q, "q_out", st);
   a.q_out_addr = addr(q_out);
   strides(a.q_out_stride, q_out);
   a.v_addr = addr(val);
@@ -220,29 +256,28 @@ PyObject* rope_append(PyObject* const* v) {
     a.k_out_addr = addr(k_out);
     strides(a.k_out_stride, k_out);
   }
-  if (const int rc = akili_rope_append(&a, stream_of(v[11]))) refuse("rope_append", rc);
+  if (const int rc = akili_rope_append(&a, st.handle())) refuse("rope_append", rc);
   return THPVariable_Wrap(q_out);
 }
 
-// (out, scaling, base, factor, original_positions, low, high, amplitude, stream)
+// (max_positions, rot_dim, scaling, base, factor, original_positions, low, high, amplitude, stream)
 PyObject* rope_table(PyObject* const* v) {
   akili_rope_table_arg_t a = {};
-  const at::Tensor& t = tensor(v[0], "out");
-  on_device(t);
-  if (t.dim() != 2 || t.scalar_type() != at::kFloat || !t.is_contiguous())
-    fail(PyExc_ValueError, "the table is a contiguous fp32 [max_positions, rot_dim] tensor");
+  const CallStream st(v[9]);
+  const at::Tensor t = st.empty({integer(v[0]), integer(v[1])},
+                                at::TensorOptions(at::kFloat).device(at::kCUDA, c10::cuda::current_device()));
   a.max_positions = size32(t.size(0), "max_positions");
   a.rot_dim = size32(t.size(1), "rot_dim");
-  a.scaling = static_cast<uint32_t>(integer(v[1]));
-  a.base = number(v[2]);
-  a.factor = number(v[3]);
-  a.original_positions = number(v[4]);
-  a.low = number(v[5]);
-  a.high = number(v[6]);
-  a.amplitude = number(v[7]);
+  a.scaling = static_cast<uint32_t>(integer(v[2]));
+  a.base = number(v[3]);
+  a.factor = number(v[4]);
+  a.original_positions = number(v[5]);
+  a.low = number(v[6]);
+  a.high = number(v[7]);
+  a.amplitude = number(v[8]);
   a.table_addr = addr(t);
-  if (const int rc = akili_rope_table(&a, stream_of(v[8]))) refuse("rope_table", rc);
-  Py_RETURN_NONE;
+  if (const int rc = akili_rope_table(&a, st.handle())) refuse("rope_table", rc);
+  return THPVariable_Wrap(t);
 }
 
 float scale_of(PyObject* o) { return o == Py_None ? 0.0f : static_cast<float>(number(o)); }
@@ -268,9 +303,10 @@ PyObject* prompt_attention(PyObject* const* v) {
   a.cu_q_addr = index(cu_q, q, {-1}, "cu_q");
   a.cu_k_addr = index(cu_k, q, {cu_q.size(0)}, "cu_k");
   if (cu_q.size(0) == 0) fail(PyExc_ValueError, "cu_q has batch + 1 entries");
-  const at::Tensor out = given_or_like(v[7], q, "out");
+  const CallStream st(v[9]);
+  const at::Tensor out = given_or_like(v[7], q, "out", st);
   at::Tensor lse;
-  if (truth(v[8])) lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+  if (truth(v[8])) lse = st.empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
   a.dtype = element(q);
   a.q_heads = size32(q.size(1), "q_heads");
   a.kv_heads = size32(k.size(1), "kv_heads");
@@ -289,7 +325,7 @@ PyObject* prompt_attention(PyObject* const* v) {
   strides(a.k_stride, k);
   strides(a.v_stride, val);
   strides(a.o_stride, out);
-  if (const int rc = akili_prompt_attention(&a, stream_of(v[9]))) refuse("prompt_attention", rc);
+  if (const int rc = akili_prompt_attention(&a, st.handle())) refuse("prompt_attention", rc);
   return with_lse(out, lse);
 }
 
@@ -304,9 +340,10 @@ PyObject* tree_mask(PyObject* const* v) {
   a.mask_words = size32(integer(v[2]), "mask_words");
   a.batch = size32(cu_q.size(0) - 1, "batch");
   a.total_q = size32(parents.size(0), "total_q");
-  const at::Tensor mask = at::empty({parents.size(0), static_cast<int64_t>(a.mask_words)}, parents.options());
+  const CallStream st(v[3]);
+  const at::Tensor mask = st.empty({parents.size(0), static_cast<int64_t>(a.mask_words)}, parents.options());
   a.mask_addr = addr(mask);
-  if (const int rc = akili_tree_mask(&a, stream_of(v[3]))) refuse("tree_mask", rc);
+  if (const int rc = akili_tree_mask(&a, st.handle())) refuse("tree_mask", rc);
   return THPVariable_Wrap(mask);
 }
 
@@ -345,9 +382,10 @@ PyObject* tree_attention(PyObject* const* v) {
     a.mask_words = size32(mask.size(1), "mask_words");
     a.mask_stride = mask.stride(0);
   }
-  const at::Tensor out = given_or_like(v[8], q, "out");
+  const CallStream st(v[11]);
+  const at::Tensor out = given_or_like(v[8], q, "out", st);
   at::Tensor lse;
-  if (truth(v[9])) lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+  if (truth(v[9])) lse = st.empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
   if (v[10] != Py_None) {
     const at::Tensor& ws = tensor(v[10], "workspace");
     if (ws.device() != q.device() || !ws.is_contiguous())
@@ -365,7 +403,7 @@ PyObject* tree_attention(PyObject* const* v) {
   strides(a.o_stride, out);
   strides(a.k_page_stride, kp);
   strides(a.v_page_stride, vp);
-  if (const int rc = akili_tree_attention(&a, stream_of(v[11]))) refuse("tree_attention", rc);
+  if (const int rc = akili_tree_attention(&a, st.handle())) refuse("tree_attention", rc);
   return with_lse(out, lse);
 }
 
@@ -393,7 +431,8 @@ PyObject* cache_accept(PyObject* const* v) {
   a.page_table_addr = index(table, kp, {lens.size(0), -1}, "page_table");
   a.accepted_addr = index(acc, kp, {lens.size(0), -1}, "accepted");
   a.n_accepted_addr = index(tensor(v[5], "n_accepted"), kp, {lens.size(0)}, "n_accepted");
-  const at::Tensor out = v[6] == Py_None ? at::empty(lens.sizes(), lens.options()) : tensor(v[6], "new_lens");
+  const CallStream st(v[7]);
+  const at::Tensor out = v[6] == Py_None ? st.empty(lens.sizes(), lens.options()) : tensor(v[6], "new_lens");
   a.new_lens_addr = index(out, kp, {lens.size(0)}, "new_lens");
   a.elem_bytes = static_cast<uint32_t>(kp.element_size());
   a.layers = lead ? size32(kp.size(0), "layers") : 1;
@@ -412,7 +451,7 @@ PyObject* cache_accept(PyObject* const* v) {
     a.k_page_stride[i] = i - 1 + lead < 0 ? 0 : kp.stride(i - 1 + lead);
     a.v_page_stride[i] = i - 1 + lead < 0 ? 0 : vp.stride(i - 1 + lead);
   }
-  if (const int rc = akili_cache_accept(&a, stream_of(v[7]))) refuse("cache_accept", rc);
+  if (const int rc = akili_cache_accept(&a, st.handle())) refuse("cache_accept", rc);
   return THPVariable_Wrap(out);
 }
 
@@ -444,7 +483,7 @@ PyMethodDef method(const char* name) {
 
 PyMethodDef methods[] = {method<rope, 9>("rope"),
                          method<rope_append, 12>("rope_append"),
-                         method<rope_table, 9>("rope_table"),
+                         method<rope_table, 10>("rope_table"),
                          method<prompt_attention, 10>("prompt_attention"),
                          method<tree_mask, 4>("tree_mask"),
                          method<tree_attention, 12>("tree_attention"),

@@ -14,7 +14,9 @@ Tensors are CUDA tensors on the current device, of any strides with a
 contiguous last axis; index tensors are int32 (slots int64).  Wrong types,
 shapes or devices raise TypeError or ValueError before the launch; the C
 entry's own refusals raise ``abi.AkiliError``.  Calls run on ``stream``
-(default: the current stream) and do not synchronise.
+(default: the current stream) and do not synchronise; what they return is
+allocated on that stream, so a stream whose inputs are ready needs to wait for
+nothing else.
 """
 from __future__ import annotations
 
@@ -45,13 +47,6 @@ class _Native:
 _native = _Native()
 
 
-def _on(stream, given: bool, result):
-    """Tell the allocator that a tensor made on the current stream is used on `stream`."""
-    if stream is not None and not given:
-        result.record_stream(stream)
-    return result
-
-
 def rope_table(max_positions: int, rot_dim: int, base: float = 10000.0, scaling: str | None = None,
                factor: float = 1.0, original_positions: float = 0.0, low: float = 0.0, high: float = 0.0,
                amplitude: float = 0.0, device=None, stream=None) -> torch.Tensor:
@@ -66,9 +61,11 @@ def rope_table(max_positions: int, rot_dim: int, base: float = 10000.0, scaling:
     and 0.1 ln(factor) + 1 for "ramp"."""
     if scaling not in abi.ROPE_SCALINGS:
         raise ValueError(f"unknown scaling {scaling!r}")
-    out = torch.empty((max_positions, rot_dim), device=device or "cuda", dtype=torch.float32)
-    _native.rope_table(out, abi.ROPE_SCALINGS[scaling], base, factor, original_positions, low, high, amplitude, stream)
-    return _on(stream, False, out)
+    place = torch.device("cuda" if device is None else device)
+    if place.type != "cuda" or place.index not in (None, torch.cuda.current_device()):
+        raise ValueError("serving ops take CUDA tensors on the current device")
+    return _native.rope_table(max_positions, rot_dim, abi.ROPE_SCALINGS[scaling], base, factor, original_positions, low,
+                              high, amplitude, stream)
 
 
 def rope(q, k, positions, table, interleaved: bool = False, inverse: bool = False, q_out=None, k_out=None,
@@ -78,8 +75,7 @@ def rope(q, k, positions, table, interleaved: bool = False, inverse: bool = Fals
 
     Pairs are (i, i + rot_dim/2), or (2i, 2i + 1) when interleaved.  inverse=True rotates back: it is the
     gradient (apply it to dq, dk).  q_out/k_out may be q/k (in place).  Returns (q_out, k_out)."""
-    qo, ko = _native.rope(q, k, positions, table, interleaved, inverse, q_out, k_out, stream)
-    return _on(stream, q_out is not None, qo), _on(stream, k_out is not None, ko)
+    return _native.rope(q, k, positions, table, interleaved, inverse, q_out, k_out, stream)
 
 
 def rope_append(q, k, v, positions, table, slots, k_pages, v_pages, interleaved: bool = False, q_out=None,
@@ -88,18 +84,7 @@ def rope_append(q, k, v, positions, table, slots, k_pages, v_pages, interleaved:
     page_size + offset (int64; -1: padding, nothing is written) of k_pages/v_pages [num_pages, page_size,
     k_heads, head_dim].  k_out, if given, gets the rotated k as well (`prompt_attention` of the same prompt
     reads it; it may be k).  Returns the rotated q (q_out; may be q)."""
-    return _on(stream, q_out is not None,
-               _native.rope_append(q, k, v, positions, table, slots, k_pages, v_pages, interleaved, q_out, k_out,
-                                   stream))
-
-
-def _attention_result(got, out, return_lse, stream):
-    if stream is not None:
-        if out is None:
-            (got[0] if return_lse else got).record_stream(stream)
-        if return_lse:
-            got[1].record_stream(stream)
-    return got
+    return _native.rope_append(q, k, v, positions, table, slots, k_pages, v_pages, interleaved, q_out, k_out, stream)
 
 
 def prompt_attention(q, k, v, cu_q, cu_k=None, softmax_scale: float | None = None, causal: bool = True, out=None,
@@ -110,15 +95,14 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, softmax_scale: float | None = Non
     With n queries and m keys, query i sees the keys j <= i + m - n (causal) or all; one that sees none gives
     0.  Query head h reads key head h // (q_heads // kv_heads).  softmax_scale defaults to head_dim**-0.5.
     Returns out, or (out, lse) with lse fp32 [total_q, q_heads] (natural log, -inf for a row without keys)."""
-    got = _native.prompt_attention(q, k, v, cu_q, cu_k, softmax_scale, causal, out, return_lse, stream)
-    return _attention_result(got, out, return_lse, stream)
+    return _native.prompt_attention(q, k, v, cu_q, cu_k, softmax_scale, causal, out, return_lse, stream)
 
 
 def tree_mask(parents, cu_q, max_nodes: int, stream=None) -> torch.Tensor:
     """The mask `tree_attention` takes, int32 [total_q, ceil(max_nodes / 32)]: bit j of node i's row is set for
     i itself and its ancestors.  parents int32 [total_q]: the parent's index within its own tree, smaller than
     the node's, or -1 for a root.  max_nodes: at least the largest tree's nodes."""
-    return _on(stream, False, _native.tree_mask(parents, cu_q, (max_nodes + 31) // 32, stream))
+    return _native.tree_mask(parents, cu_q, (max_nodes + 31) // 32, stream)
 
 
 def tree_attention(q, k_pages, v_pages, page_table, context_lens, cu_q, mask=None, softmax_scale: float | None = None,
@@ -131,9 +115,8 @@ def tree_attention(q, k_pages, v_pages, page_table, context_lens, cu_q, mask=Non
     head_dim] (any strides, page_size a multiple of 8).  Every new token sees the context and the new tokens
     of its mask row (`tree_mask`); without a mask, itself and those before it (a single token, a chunk).
     Returns out, or (out, lse); `workspace` is an optional uint8 tensor of tree_attention_workspace() bytes."""
-    got = _native.tree_attention(q, k_pages, v_pages, page_table, context_lens, cu_q, mask, softmax_scale, out,
-                                 return_lse, workspace, stream)
-    return _attention_result(got, out, return_lse, stream)
+    return _native.tree_attention(q, k_pages, v_pages, page_table, context_lens, cu_q, mask, softmax_scale, out,
+                                  return_lse, workspace, stream)
 
 
 def tree_attention_workspace(q, k_pages, page_table, context_lens) -> int:
@@ -148,5 +131,4 @@ def cache_accept(k_pages, v_pages, page_table, context_lens, accepted, n_accepte
     in place: entry context_lens[b] + accepted[b, i] of sequence b moves to context_lens[b] + i for i <
     n_accepted[b].  accepted int32 [batch, any] ascends in each row.  Returns context_lens + n_accepted
     (new_lens, not context_lens itself)."""
-    return _on(stream, new_lens is not None,
-               _native.cache_accept(k_pages, v_pages, page_table, context_lens, accepted, n_accepted, new_lens, stream))
+    return _native.cache_accept(k_pages, v_pages, page_table, context_lens, accepted, n_accepted, new_lens, stream)

@@ -8,6 +8,9 @@ from akili_bench_b200 import ops  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
+F16, BF16 = torch.float16, torch.bfloat16
+i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+
 
 @pytest.fixture(autouse=True)
 def clean_status():
@@ -22,3 +25,99 @@ def test_warps_that_share_a_barrier_give_up_together(limit_us):
     for the other at their next barrier); the status would be STATUS_SELFTEST_SHARED."""
     ops.selftest_wait_timeout(limit_us)
     assert ops.device_status() == ops.STATUS_SELFTEST
+
+
+# ------------------------------------------------------- streams and graphs --
+TOKENS, HEADS, DIM = 1024, 32, 128
+
+
+def side_calls():
+    """name -> (call on a stream, bytes of its result), on inputs that are ready."""
+    q = torch.randn(TOKENS, HEADS, DIM, device="cuda", dtype=F16)
+    none = q[:, :0]
+    positions = torch.arange(TOKENS, dtype=torch.int32, device="cuda")
+    table = ops.rope_table(TOKENS, DIM)
+    pages, v_pages = (torch.zeros(TOKENS // 16, 16, 1, DIM, device="cuda", dtype=F16) for _ in range(2))
+    out = torch.empty_like(q)
+    slots = torch.arange(TOKENS, device="cuda")
+    cu, lens = i32([0, TOKENS]), i32([0])
+    page_table = torch.arange(TOKENS // 16, dtype=torch.int32, device="cuda")[None]
+    parents = torch.arange(TOKENS, dtype=torch.int32, device="cuda") - 1
+    many = torch.zeros(1 << 15, dtype=torch.int32, device="cuda")
+    one_page, v_page = (torch.zeros(1, 8, 1, 8, device="cuda", dtype=F16) for _ in range(2))
+    wide = torch.zeros(1 << 15, 1, dtype=torch.int32, device="cuda")
+    of = lambda t: t[0] if isinstance(t, tuple) else t  # noqa: E731
+    return {
+        "rope": (lambda s: of(ops.rope(q, none, positions, table, stream=s)), q.nbytes),
+        "rope_append": (lambda s: ops.rope_append(q, q[:, :1], q[:, :1], positions, table, slots, pages, v_pages,
+                                                  stream=s), q.nbytes),
+        "rope_table": (lambda s: ops.rope_table(TOKENS, DIM, stream=s), TOKENS * DIM * 4),
+        "prompt_attention": (lambda s: ops.prompt_attention(q, q, q, cu, stream=s), q.nbytes),
+        "prompt_lse": (lambda s: ops.prompt_attention(q, q, q, cu, out=out, return_lse=True, stream=s)[1],
+                       TOKENS * HEADS * 4),
+        "tree_attention": (lambda s: ops.tree_attention(q, pages, pages, page_table, lens, cu, stream=s), q.nbytes),
+        "tree_mask": (lambda s: ops.tree_mask(parents, cu, TOKENS, stream=s), TOKENS * TOKENS // 8),
+        "cache_accept": (lambda s: ops.cache_accept(one_page, v_page, wide, many, wide, many, stream=s),
+                         many.nbytes),
+    }
+
+
+@pytest.mark.parametrize("name", ["rope", "rope_append", "rope_table", "prompt_attention", "prompt_lse",
+                                  "tree_attention", "tree_mask", "cache_accept"])
+def test_results_on_another_stream_do_not_take_memory_that_is_still_in_use(name):
+    """A block freed on the current stream, while what is queued there has yet to read it, is not the result of a
+    call on a stream that waits for nothing."""
+    call, size = side_calls()[name]
+    side = torch.cuda.Stream()
+    call(side)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    blocks = [torch.full((size,), 7, dtype=torch.uint8, device="cuda") for _ in range(4)]
+    kept = [torch.zeros_like(b) for b in blocks]
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100_000_000)  # some 50 ms
+    for b, k in zip(blocks, kept):
+        k.copy_(b)
+    freed = {b.data_ptr() for b in blocks}
+    del blocks, b, k
+    result = call(side)
+    assert result.data_ptr() not in freed
+    torch.cuda.synchronize()
+    assert all((k == 7).all() for k in kept)
+
+
+def test_results_on_another_stream_outlive_what_the_callers_stream_does_with_them():
+    """Freed while the caller's stream has yet to read it, a result's memory does not go to that stream's next call."""
+    call, size = side_calls()["rope"]
+    side = torch.cuda.Stream()
+    result = call(side)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda._sleep(100_000_000)
+    kept = result.clone()
+    freed = result.data_ptr()
+    del result
+    later = call(side)
+    assert later.data_ptr() != freed
+    torch.cuda.synchronize()
+    assert torch.equal(kept, later)
+
+
+def test_streams_of_other_kinds():
+    q = torch.randn(4, 2, 64, device="cuda", dtype=F16)
+    cu = i32([0, 4])
+    want = ops.prompt_attention(q, q, q, cu)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    raw = type("Raw", (), {"cuda_stream": side.cuda_stream})()
+    for s in (side, raw, torch.cuda.ExternalStream(side.cuda_stream), torch.cuda.default_stream()):
+        got = ops.prompt_attention(q, q, q, cu, stream=s)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    with torch.cuda.stream(side):
+        got = ops.prompt_attention(q, q, q, cu, stream=torch.cuda.default_stream())
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    with pytest.raises(ValueError):
+        ops.prompt_attention(q, q, q, cu, stream=torch.Stream("cpu"))
+    with pytest.raises(AttributeError):
+        ops.prompt_attention(q, q, q, cu, stream=3)
