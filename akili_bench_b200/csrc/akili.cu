@@ -212,13 +212,25 @@ int current_context_id(unsigned long long* id) {
 // --------------------------------------------------------------- scratch --
 // Internal scratch, one grow-only buffer per (context, stream): calls on one
 // stream are ordered, so they can share it.  Used when the caller gives no
-// akili_ex_t workspace.  Growing it frees the old buffer (a device sync).
+// akili_ex_t workspace.  Growing it frees the old buffer (a device sync),
+// unless a call was captured with it: the graph's kernels go on using it, so
+// it is kept.
 // cudaStreamPerThread names a different stream in every host thread, so for
 // it the calling thread is part of the key.
 struct Pool {
   void* ptr = nullptr;
   size_t bytes = 0;
+  bool captured = false;
 };
+
+bool is_capturing(cudaStream_t st) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(st, &status) != cudaSuccess) {
+    cudaGetLastError();  // (the legacy stream beside a capture: the launch is refused)
+    return false;
+  }
+  return status == cudaStreamCaptureStatusActive;
+}
 
 int pool_get(cudaStream_t st, size_t bytes, void** out) {
   static std::mutex mu;
@@ -230,9 +242,8 @@ int pool_get(cudaStream_t st, size_t bytes, void** out) {
   std::lock_guard<std::mutex> g(mu);
   Pool& p = pools[{ctx, st, owner}];
   if (p.bytes < bytes) {
-    if (p.ptr) cudaFree(p.ptr);
-    p.ptr = nullptr;
-    p.bytes = 0;
+    if (p.ptr && !p.captured) cudaFree(p.ptr);
+    p = Pool{};
     size_t want = bytes + bytes / 4 + (1u << 20);
     if (cudaMalloc(&p.ptr, want) != cudaSuccess) {
       cudaGetLastError();
@@ -240,6 +251,7 @@ int pool_get(cudaStream_t st, size_t bytes, void** out) {
     }
     p.bytes = want;
   }
+  if (is_capturing(st)) p.captured = true;
   *out = p.ptr;
   return AKILI_OK;
 }

@@ -12,6 +12,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Stream.h>
@@ -141,6 +142,9 @@ class CallStream {
     const c10::cuda::CUDAStream s = given(o, caller_.device_index());
     handle_ = s.stream();
     if (handle_ != caller_.stream()) guard_.emplace(s);
+  }
+  bool capturing() const {  // (the call's stream is the current one)
+    return c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
   }
   akili_stream_t handle() const { return reinterpret_cast<akili_stream_t>(handle_); }
   at::Tensor empty(at::IntArrayRef sizes, const at::TensorOptions& options) const {
@@ -386,10 +390,19 @@ PyObject* tree_attention(PyObject* const* v) {
   const at::Tensor out = given_or_like(v[8], q, "out", st);
   at::Tensor lse;
   if (truth(v[9])) lse = st.empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+  at::Tensor ws;
   if (v[10] != Py_None) {
-    const at::Tensor& ws = tensor(v[10], "workspace");
+    ws = tensor(v[10], "workspace");
     if (ws.device() != q.device() || !ws.is_contiguous())
       fail(PyExc_ValueError, "workspace is a contiguous tensor on the device of q");
+  } else if (st.capturing()) {
+    // A graph's own memory: the stream's scratch belongs to its eager calls,
+    // which a replay on another stream would not be ordered with.
+    uint64_t n = 0;
+    if (const int rc = akili_tree_attention_workspace(&a, &n)) refuse("tree_attention", rc);
+    ws = st.empty({static_cast<int64_t>(n)}, q.options().dtype(at::kByte));
+  }
+  if (ws.defined()) {
     a.workspace = addr(ws);
     a.workspace_bytes = static_cast<uint64_t>(ws.nbytes());
   }

@@ -142,7 +142,11 @@ int akili_prompt_attention(const akili_prompt_attention_arg_t* arg, akili_stream
  * prompt).  Otherwise as akili_prompt_attention.  Pages or page rows past a
  * sequence's end may hold anything; table entries past it are not read.  A page
  * index outside [0, num_pages) reads as a page of zeros; a sequence is clamped
- * to max_pages * page_size entries; both are recorded. */
+ * to max_pages * page_size entries; both are recorded.
+ * Without a workspace the call uses the scratch of its stream.  A graph that
+ * was captured so keeps that memory for good, and its replays have to be
+ * ordered with the stream's other calls; with a workspace of its own it is
+ * independent of them. */
 typedef struct {
   uint32_t dtype; /* F16 or BF16 */
   uint32_t q_heads, kv_heads, head_dim;

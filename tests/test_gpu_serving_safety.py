@@ -1,10 +1,12 @@
 """The serving operators where calls meet: waits that give up, streams, captured
 graphs, buffers that overlap, requests a default could hide."""
+import ctypes as C
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
-from akili_bench_b200 import ops  # noqa: E402
+from akili_bench_b200 import abi, ops  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -121,3 +123,69 @@ def test_streams_of_other_kinds():
         ops.prompt_attention(q, q, q, cu, stream=torch.Stream("cpu"))
     with pytest.raises(AttributeError):
         ops.prompt_attention(q, q, q, cu, stream=3)
+
+
+def step(tokens, group, context, dtype=F16, pages=64):
+    """Arguments of a tree_attention call of `tokens` new tokens for each of two sequences."""
+    q = torch.randn(2 * tokens, group, 128, device="cuda", dtype=dtype)
+    kp, vp = (torch.randn(2 * pages, 16, 1, 128, device="cuda", dtype=dtype) for _ in range(2))
+    table = torch.randperm(2 * pages, device="cuda").to(torch.int32).view(2, pages)
+    return q, kp, vp, table, i32([context, context // 3]), i32([0, tokens, 2 * tokens])
+
+
+def c_entry(args, out, stream, workspace=None):
+    """akili_tree_attention itself, without the torch front end."""
+    q, kp, vp, table, lens, cu = args
+    a = abi.TreeAttentionArg(abi.DTYPE_F16, q.shape[1], 1, 128, 2, q.shape[0], kp.shape[0], 16, table.shape[1], 0, 0.0, 0,
+                             q.data_ptr(), kp.data_ptr(), vp.data_ptr(), out.data_ptr(), 0, table.data_ptr(),
+                             lens.data_ptr(), cu.data_ptr(), 0, 0, 0, *q.stride()[:2], *out.stride()[:2],
+                             *kp.stride()[:3], *vp.stride()[:3], table.stride(0), 0)
+    if workspace is not None:
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.nbytes
+    assert abi.load().akili_tree_attention(C.byref(a), stream.cuda_stream) == abi.OK
+
+
+@pytest.mark.parametrize("front_end", [True, False])
+def test_a_captured_step_outlives_the_growth_of_the_streams_scratch(front_end):
+    """Captured in the 16-row form without a workspace; the 256-row form then needs a larger scratch on the same
+    stream, and the memory that this frees is taken by others."""
+    small, large = step(1, 8, 900), step(60, 8, 700)
+    want, want_large = (ops.tree_attention(*s, workspace=torch.empty(64 << 20, dtype=torch.uint8, device="cuda"))
+                        for s in (small, large))
+    out = torch.zeros_like(want)
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    call = (lambda: ops.tree_attention(*small, out=out)) if front_end else (lambda: c_entry(small, out, side))
+    with torch.cuda.stream(side):
+        call()  # the scratch of this stream, sized for the small step
+        side.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            call()
+        out.zero_()
+        assert torch.equal(ops.tree_attention(*large), want_large)
+        junk = [torch.full((n << 20,), 255, dtype=torch.uint8, device="cuda") for n in (1, 2, 3, 4, 5, 8)]
+        graph.replay()
+        side.synchronize()
+    assert torch.equal(out, want)
+    assert all((j == 255).all() for j in junk)
+
+
+def test_a_captured_step_shares_no_memory_with_the_streams_eager_calls():
+    """Replays on one stream beside eager calls on the stream of the capture."""
+    captured, eager = step(1, 8, 1000), step(3, 2, 800)
+    want, want_eager = ops.tree_attention(*captured), ops.tree_attention(*eager)
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    out = torch.zeros_like(want)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):  # (no eager call before it)
+        ops.tree_attention(*captured, out=out)
+    torch.cuda.synchronize()
+    for _ in range(50):
+        with torch.cuda.stream(other):
+            graph.replay()
+        with torch.cuda.stream(side):
+            got = [ops.tree_attention(*eager) for _ in range(3)]
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and all(torch.equal(x, want_eager) for x in got)
