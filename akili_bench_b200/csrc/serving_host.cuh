@@ -212,6 +212,16 @@ int run_tree_mask(const akili_tree_mask_arg_t* a, cudaStream_t st) {
                           static_cast<int>(a->total_q), static_cast<int>(a->mask_words));
 }
 
+// Whether the int32s of `a` [rows, cols] share memory with the n at `p`.
+bool ints_overlap(uint64_t a, uint64_t rows, uint64_t cols, int64_t row_stride, uint64_t p, uint64_t n) {
+  if (a == 0 || p == 0) return false;
+  for (uint64_t r = 0; r < rows; ++r) {
+    const uint64_t row = a + 4 * static_cast<int64_t>(r) * row_stride;
+    if (row < p + 4 * n && p < row + 4 * cols) return true;
+  }
+  return false;
+}
+
 template <typename U>
 int launch_accept(AcceptArgs g, const akili_cache_accept_arg_t* a, cudaStream_t st) {
   g.vecs = static_cast<int>(a->head_dim * a->elem_bytes / sizeof(U));
@@ -235,7 +245,12 @@ int run_cache_accept(const akili_cache_accept_arg_t* a, cudaStream_t st) {
   if ((rc = check_aligned({a->page_table_addr, a->context_lens_addr, a->n_accepted_addr}, 4))) return rc;
   if (a->max_accepted && (rc = check_aligned({a->accepted_addr}, 4))) return rc;
   if (a->new_lens_addr % 4) return AKILI_E_ALIGN;
-  if (a->new_lens_addr == a->context_lens_addr) return AKILI_E_UNSUPPORTED;
+  // one block writes a sequence's new length while others still read what the moves go by
+  const uint64_t out = a->new_lens_addr, n = a->batch;
+  if (ints_overlap(a->context_lens_addr, 1, n, 0, out, n) || ints_overlap(a->n_accepted_addr, 1, n, 0, out, n) ||
+      ints_overlap(a->accepted_addr, n, a->max_accepted, a->accepted_stride, out, n) ||
+      ints_overlap(a->page_table_addr, n, a->max_pages, a->page_table_stride, out, n))
+    return AKILI_E_UNSUPPORTED;
   DevInfo di;
   if ((rc = device_info(&di))) return rc;
   AcceptArgs g{};

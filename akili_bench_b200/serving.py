@@ -130,5 +130,5 @@ def cache_accept(k_pages, v_pages, page_table, context_lens, accepted, n_accepte
     k_pages/v_pages [layers, num_pages, page_size, kv_heads, head_dim] (or without the layers axis) are changed
     in place: entry context_lens[b] + accepted[b, i] of sequence b moves to context_lens[b] + i for i <
     n_accepted[b].  accepted int32 [batch, any] ascends in each row.  Returns context_lens + n_accepted
-    (new_lens, not context_lens itself)."""
+    (new_lens, which shares no memory with the index tensors)."""
     return _native.cache_accept(k_pages, v_pages, page_table, context_lens, accepted, n_accepted, new_lens, stream)

@@ -204,7 +204,7 @@ typedef struct {
   uint64_t context_lens_addr; /* int32 [batch] */
   uint64_t accepted_addr;     /* int32 [batch, max_accepted] */
   uint64_t n_accepted_addr;   /* int32 [batch] */
-  uint64_t new_lens_addr;     /* optional int32 [batch]; not context_lens itself */
+  uint64_t new_lens_addr;     /* optional int32 [batch]; shares no memory with the four above */
   int64_t  k_page_stride[4], v_page_stride[4]; /* layer, page, token, head */
   int64_t  page_table_stride, accepted_stride;
 } akili_cache_accept_arg_t;

@@ -189,3 +189,16 @@ def test_a_captured_step_shares_no_memory_with_the_streams_eager_calls():
             got = [ops.tree_attention(*eager) for _ in range(3)]
         torch.cuda.synchronize()
         assert torch.equal(out, want) and all(torch.equal(x, want_eager) for x in got)
+
+
+# ------------------------------------------------------------------- accept --
+def test_cache_accept_refuses_to_write_lengths_over_its_inputs():
+    pages = torch.zeros(2, 4, 8, 1, 8, device="cuda", dtype=F16)
+    ints = torch.zeros(4, 16, dtype=torch.int32, device="cuda")
+    table, lens, accepted, n = ints[:2, :2], ints[2, :2], ints[:2, 4:6], ints[3, :2]
+    for out in (lens, n, ints[2, 1:3], ints[3, 1:3], ints[0, 4:6], ints[1, 1:3], ints[1, 5:7]):
+        with pytest.raises(abi.AkiliError) as e:
+            ops.cache_accept(pages, pages.clone(), table, lens, accepted, n, new_lens=out)
+        assert e.value.code == abi.E_UNSUPPORTED
+    for out in (ints[3, 2:4], ints[0, 2:4], ints[0, 6:8]):  # (between the rows of the page table and of accepted)
+        assert ops.cache_accept(pages, pages.clone(), table, lens, accepted, n, new_lens=out).tolist() == [0, 0]

@@ -152,6 +152,24 @@ def test_cache_accept_refusals(change, want):
     assert code("cache_accept", a) == want
 
 
+@pytest.mark.parametrize("read,cols,stride", [("context_lens", 1, 0), ("n_accepted", 1, 0), ("accepted", 8, 11),
+                                              ("page_table", 7, 11)])
+def test_cache_accept_refuses_new_lengths_over_what_it_reads(read, cols, stride):
+    """New lengths (batch int32) that share even four bytes with an index tensor; next to it they are taken."""
+    torch = pytest.importorskip("torch")
+    batch = 3
+    first, last = (0, 4 * (batch - 1)) if stride == 0 else (0, 4 * ((batch - 1) * stride + cols - 1))
+    for at, refused in ((first, True), (last, True), (first - 4 * (batch - 1), True), (first - 4 * batch, False),
+                        (last + 4, False), (4 * cols, stride == 0)):
+        a = abi.CacheAcceptArg(2, 4, batch, 2, 64, 50, 16, 7, 8, 0, A, A, 2 * A, 3 * A, 4 * A, 5 * A, 0, 102400, 2048, 128,
+                               64, 102400, 2048, 128, 64, 11, 11)
+        a.new_lens_addr = getattr(a, read + "_addr") + at
+        if refused:
+            assert code("cache_accept", a) == abi.E_UNSUPPORTED, (read, at)
+        elif not torch.cuda.is_available():  # (with a GPU it would run, on addresses that are none)
+            assert code("cache_accept", a) == abi.E_NO_DEVICE, (read, at)
+
+
 def test_valid_blocks_without_a_gpu_report_no_device():
     torch = pytest.importorskip("torch")
     if torch.cuda.is_available():
