@@ -33,7 +33,7 @@ namespace akili {
 
 constexpr int kRopeThreads = 64;
 
-__device__ __forceinline__ void record_bad_index() { atomicCAS(&g_status, 0u, AKILI_STATUS_BAD_INDEX); }
+static_assert(kStatusBadIndex == AKILI_STATUS_BAD_INDEX, "status code of a skipped index");
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }

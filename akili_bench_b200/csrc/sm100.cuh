@@ -17,10 +17,12 @@
 namespace akili {
 
 // ---------------------------------------------------------------- status --
-// First device-side wait that ran out of time (0 = none).  Read by
+// First device-side wait that ran out of time, or if none did kStatusBadIndex
+// once an index out of range was skipped (0 = neither).  Read by
 // akili_device_status(); every wait is bounded so a broken pipeline ends the
 // kernel instead of hanging the GPU.
 __device__ unsigned int g_status;
+constexpr unsigned int kStatusBadIndex = 0x2001u;
 constexpr unsigned long long kWaitTimeoutNs = 2000000000ull;  // 2 s per wait
 
 enum WaitSite : uint32_t {
@@ -61,8 +63,9 @@ __device__ __forceinline__ bool kclock_thread() {
   return blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0;
 }
 __device__ __forceinline__ void record_timeout(uint32_t site) {
-  atomicCAS(&g_status, 0u, 0x1000u | site);
+  if (atomicCAS(&g_status, 0u, 0x1000u | site) == kStatusBadIndex) atomicCAS(&g_status, kStatusBadIndex, 0x1000u | site);
 }
+__device__ __forceinline__ void record_bad_index() { atomicCAS(&g_status, 0u, kStatusBadIndex); }
 
 __device__ __forceinline__ KClock kclock_begin() {
   KClock k{0, 0};

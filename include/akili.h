@@ -463,9 +463,12 @@ int akili_workspace_bytes(const char* op, const void* arg, const akili_ex_t* ex,
  * device are serialised by a lock. */
 int akili_host_call(const char* op, const void* arg, const akili_ex_t* ex, akili_stream_t stream);
 
-/* Device status word of the current device: 0 when no kernel has timed out
- * on a device-side wait since the last clear, else the code of the first wait
- * that gave up.  Synchronises the device. `clear` != 0 resets it. */
+/* Device status word of the current device.  Where a kernel has timed out on
+ * a device-side wait since the last clear: the code of the first wait that
+ * gave up, and AKILI_E_DEVICE_TIMEOUT is returned.  Else, where a serving
+ * operator has skipped an index out of range: AKILI_STATUS_BAD_INDEX
+ * (akili_serving.h), and AKILI_E_SHAPE.  Else 0, and AKILI_OK.  Synchronises
+ * the device. `clear` != 0 resets it. */
 int akili_device_status(uint32_t* status, int clear);
 
 /* Self-test of device-side failure detection: launches one CTA that waits

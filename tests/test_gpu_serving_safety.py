@@ -29,6 +29,23 @@ def test_warps_that_share_a_barrier_give_up_together(limit_us):
     assert ops.device_status() == ops.STATUS_SELFTEST
 
 
+def test_a_timeout_is_reported_after_a_skipped_index():
+    """A skipped index is survivable, a wait that gave up is not: whichever comes first, the latter is reported."""
+    q = torch.ones(2, 1, 8, device="cuda", dtype=F16)
+    table = ops.rope_table(4, 8)
+    skip = lambda: ops.rope(q, q, i32([0, 9]), table)  # noqa: E731
+    wait = lambda: ops.selftest_wait_timeout(200)  # noqa: E731
+    v = C.c_uint32(0)
+    for calls, status, rc in (((skip,), abi.STATUS_BAD_INDEX, abi.E_SHAPE),
+                              ((skip, wait), ops.STATUS_SELFTEST, abi.E_DEVICE_TIMEOUT),
+                              ((wait, skip), ops.STATUS_SELFTEST, abi.E_DEVICE_TIMEOUT),
+                              ((skip, wait, skip), ops.STATUS_SELFTEST, abi.E_DEVICE_TIMEOUT)):
+        for call in calls:
+            call()
+        assert abi.load().akili_device_status(C.byref(v), 1) == rc and v.value == status
+    assert ops.device_status() == 0
+
+
 # ------------------------------------------------------- streams and graphs --
 TOKENS, HEADS, DIM = 1024, 32, 128
 
