@@ -19,6 +19,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <initializer_list>
+#include <limits>
 #include <optional>
 #include <string>
 
@@ -284,7 +285,14 @@ PyObject* rope_table(PyObject* const* v) {
   return THPVariable_Wrap(t);
 }
 
-float scale_of(PyObject* o) { return o == Py_None ? 0.0f : static_cast<float>(number(o)); }
+// 0 stands for the default in the C entries.  A given scale that is 0 in fp32
+// becomes the smallest positive one, which weighs all visible keys alike: it
+// moves a weight by less than 2^-20 for any finite score.
+float scale_of(PyObject* o) {
+  if (o == Py_None) return 0.0f;
+  const float s = static_cast<float>(number(o));
+  return s != 0.0f ? s : std::numeric_limits<float>::denorm_min();
+}
 
 PyObject* with_lse(const at::Tensor& out, const at::Tensor& lse) {
   if (!lse.defined()) return THPVariable_Wrap(out);

@@ -93,8 +93,8 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, softmax_scale: float | None = Non
     head_dim] and the key rows cu_k[b]:cu_k[b+1] (default cu_q) of k, v [total_k, kv_heads, head_dim].
 
     With n queries and m keys, query i sees the keys j <= i + m - n (causal) or all; one that sees none gives
-    0.  Query head h reads key head h // (q_heads // kv_heads).  softmax_scale defaults to head_dim**-0.5.
-    Returns out, or (out, lse) with lse fp32 [total_q, q_heads] (natural log, -inf for a row without keys)."""
+    0.  Query head h reads key head h // (q_heads // kv_heads).  softmax_scale defaults to head_dim**-0.5;
+    0.0 weighs all visible keys alike.  Returns out, or (out, lse) with lse fp32 [total_q, q_heads] (natural log, -inf for a row without keys)."""
     return _native.prompt_attention(q, k, v, cu_q, cu_k, softmax_scale, causal, out, return_lse, stream)
 
 

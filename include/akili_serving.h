@@ -122,7 +122,7 @@ typedef struct {
   uint32_t q_heads, kv_heads, head_dim; /* q_heads % kv_heads == 0; head_dim % 8 == 0, <= 128 */
   uint32_t batch, total_q, total_k;
   uint32_t causal;        /* 0 or 1 */
-  float    softmax_scale; /* 0: head_dim^-0.5 */
+  float    softmax_scale; /* 0: head_dim^-0.5 (the smallest positive float: equal weights) */
   uint32_t reserved;      /* 0 */
   uint64_t q_addr, k_addr, v_addr, o_addr;
   uint64_t lse_addr;              /* optional fp32 [total_q, q_heads]: log of the row's sum of exponentials */

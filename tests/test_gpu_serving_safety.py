@@ -7,6 +7,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from akili_bench_b200 import abi, ops  # noqa: E402
+import serving_reference as ref  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -219,3 +220,38 @@ def test_cache_accept_refuses_to_write_lengths_over_its_inputs():
         assert e.value.code == abi.E_UNSUPPORTED
     for out in (ints[3, 2:4], ints[0, 2:4], ints[0, 6:8]):  # (between the rows of the page table and of accepted)
         assert ops.cache_accept(pages, pages.clone(), table, lens, accepted, n, new_lens=out).tolist() == [0, 0]
+
+
+# --------------------------------------------------- what a default could hide --
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-50])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 55])  # (scores up to 2^120, near the end of fp32)
+@pytest.mark.parametrize("qlens,heads", [([40, 130], 2), ([700, 300], 32)])  # one tile a CTA, two
+def test_prompt_attention_with_a_scale_of_zero(scale, size, qlens, heads):
+    g = torch.Generator().manual_seed(len(qlens) * heads)
+    q, k, v = (torch.randn(sum(qlens), heads, 64, generator=g) for _ in range(3))
+    q, k, v = (q * size).to(BF16), (k * size).to(BF16), v.to(BF16)
+    cu = [0, qlens[0], sum(qlens)]
+    got, lse = ops.prompt_attention(q.cuda(), k.cuda(), v.cuda(), i32(cu), softmax_scale=scale, return_lse=True)
+    for a, b in zip(cu, cu[1:]):
+        o, l, bound, l_bound = ref.attend(q[a:b], k[a:b], v[a:b], ref.causal(b - a, b - a), 0.0)
+        ref.assert_within(got[a:b], o, bound)
+        ref.assert_within(lse[a:b], l, l_bound)
+
+
+@pytest.mark.parametrize("new,group", [(1, 4), (5, 8), (20, 6), (70, 4)])  # 16, 64, 128 and 256 rows
+def test_tree_attention_with_a_scale_of_zero(new, group):
+    args = step(new, group, 900)
+    q, kp, vp, table, lens, cu = args
+    got = ops.tree_attention(*args, softmax_scale=0.0)
+    for b, c in enumerate(lens.tolist()):
+        k, v = (p[table[b].long()].flatten(0, 1)[:c + new].cpu() for p in (kp, vp))
+        o, _, bound, _ = ref.attend(q[b * new:(b + 1) * new].cpu(), k, v, ref.causal(new, c + new), 0.0)
+        ref.assert_within(got[b * new:(b + 1) * new], o, bound)
+
+
+def test_scales_that_are_refused():
+    q = torch.ones(4, 2, 64, device="cuda", dtype=F16)
+    for scale in (-1.0, float("nan"), float("inf"), 1e39):
+        with pytest.raises(abi.AkiliError) as e:
+            ops.prompt_attention(q, q, q, i32([0, 4]), softmax_scale=scale)
+        assert e.value.code == abi.E_UNSUPPORTED
