@@ -391,6 +391,8 @@ PyObject* tree_attention(PyObject* const* v) {
   if (v[6] != Py_None) {
     const at::Tensor& mask = tensor(v[6], "mask");
     a.mask_addr = index(mask, q, {q.size(0), -1}, "mask");
+    // (a mask of no words has no address, which would be no mask at all)
+    if (mask.size(1) == 0 && q.size(0) > 0) fail(PyExc_ValueError, "mask rows have at least one word");
     a.mask_words = size32(mask.size(1), "mask_words");
     a.mask_stride = mask.stride(0);
   }

@@ -249,6 +249,15 @@ def test_tree_attention_with_a_scale_of_zero(new, group):
         ref.assert_within(got[b * new:(b + 1) * new], o, bound)
 
 
+def test_a_mask_of_no_words_is_refused():
+    """It says that no new token sees any; without a mask they would see one another."""
+    args = step(3, 4, 100)
+    with pytest.raises(ValueError):
+        ops.tree_attention(*args, torch.zeros(6, 0, dtype=torch.int32, device="cuda"))
+    none = (args[0][:0], *args[1:5], i32([0, 0, 0]))
+    assert ops.tree_attention(*none, torch.zeros(0, 0, dtype=torch.int32, device="cuda")).shape == (0, 4, 128)
+
+
 def test_scales_that_are_refused():
     q = torch.ones(4, 2, 64, device="cuda", dtype=F16)
     for scale in (-1.0, float("nan"), float("inf"), 1e39):
