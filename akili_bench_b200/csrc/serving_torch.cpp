@@ -16,10 +16,13 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Stream.h>
+#include <torch/csrc/autograd/VariableTypeUtils.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <initializer_list>
 #include <limits>
+#include <memory>
 #include <optional>
 #include <string>
 
@@ -180,6 +183,44 @@ void strides(int64_t (&to)[n], const at::Tensor& t, int64_t from = 0) {
   for (size_t i = 0; i < n; ++i) to[i] = t.stride(from + static_cast<int64_t>(i));
 }
 
+// A tensor that was given and is written: a backward pass that saved its old
+// values has to notice.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) torch::autograd::increment_version(t);
+}
+
+// The operators have no autograd formulas.  Where an input is part of a graph
+// the results are too, behind a node that raises in a backward pass: they
+// would look like constants otherwise.  Made before the launch, which a
+// refusal (a leaf written in place, say) must not follow.
+class Untaught {
+ public:
+  Untaught(const char* name, std::initializer_list<const at::Tensor*> inputs,
+           std::initializer_list<PyObject*> given = {}) {
+    if (!at::GradMode::is_enabled()) return;
+    torch::autograd::edge_list edges;
+    for (const at::Tensor* t : inputs)
+      if (t->requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(*t));
+    if (edges.empty()) return;
+    for (PyObject* o : given)
+      if (o != Py_None) torch::autograd::check_inplace(THPVariable_Unpack(o), true);
+    node_ = std::make_shared<torch::autograd::NotImplemented>(name, std::move(edges));
+  }
+  // A result, in a tensor that was `given` or a new one.
+  void result(const at::Tensor& t, PyObject* given = Py_None) const {
+    if (given != Py_None) written(t);
+    if (!node_) return;
+    const torch::autograd::Edge edge(node_, node_->add_input_metadata(t));
+    if (given != Py_None) torch::autograd::impl::rebase_history(t, edge);
+    else torch::autograd::impl::set_gradient_edge(t, edge);
+  }
+
+ private:
+  std::shared_ptr<torch::autograd::Node> node_;
+};
+
+constexpr const char* kRopeGradient = "ops.rope (it is ops.rope of the gradients with inverse=True)";
+
 at::Tensor given_or_like(PyObject* o, const at::Tensor& like, const char* name, const CallStream& st) {
   if (o == Py_None) return st.empty(like.sizes(), like.options());
   const at::Tensor& t = tensor(o, name);
@@ -225,7 +266,10 @@ PyObject* rope(PyObject* const* v) {
   a.k_out_addr = addr(k_out);
   strides(a.q_out_stride, q_out);
   strides(a.k_out_stride, k_out);
+  const Untaught history(kRopeGradient, {&q, &k}, {v[6], v[7]});
   if (const int rc = akili_rope(&a, st.handle())) refuse("rope", rc);
+  history.result(q_out, v[6]);
+  history.result(k_out, v[7]);
   return Py_BuildValue("(NN)", THPVariable_Wrap(q_out), THPVariable_Wrap(k_out));
 }
 
@@ -261,7 +305,13 @@ PyObject* rope_append(PyObject* const* v) {
     a.k_out_addr = addr(k_out);
     strides(a.k_out_stride, k_out);
   }
+  const Untaught history("ops.rope_append", {&q, &k, &val}, {v[9], v[10]});
   if (const int rc = akili_rope_append(&a, st.handle())) refuse("rope_append", rc);
+  history.result(q_out, v[9]);
+  if (v[10] != Py_None) history.result(THPVariable_Unpack(v[10]), v[10]);
+  // (a cache that carried history would hold every step's graph)
+  written(kp);
+  written(vp);
   return THPVariable_Wrap(q_out);
 }
 
@@ -337,7 +387,10 @@ PyObject* prompt_attention(PyObject* const* v) {
   strides(a.k_stride, k);
   strides(a.v_stride, val);
   strides(a.o_stride, out);
+  const Untaught history("ops.prompt_attention", {&q, &k, &val}, {v[7]});
   if (const int rc = akili_prompt_attention(&a, st.handle())) refuse("prompt_attention", rc);
+  history.result(out, v[7]);
+  if (lse.defined()) history.result(lse);
   return with_lse(out, lse);
 }
 
@@ -426,7 +479,10 @@ PyObject* tree_attention(PyObject* const* v) {
   strides(a.o_stride, out);
   strides(a.k_page_stride, kp);
   strides(a.v_page_stride, vp);
+  const Untaught history("ops.tree_attention", {&q, &kp, &vp}, {v[8]});
   if (const int rc = akili_tree_attention(&a, st.handle())) refuse("tree_attention", rc);
+  history.result(out, v[8]);
+  if (lse.defined()) history.result(lse);
   return with_lse(out, lse);
 }
 
@@ -475,6 +531,9 @@ PyObject* cache_accept(PyObject* const* v) {
     a.v_page_stride[i] = i - 1 + lead < 0 ? 0 : vp.stride(i - 1 + lead);
   }
   if (const int rc = akili_cache_accept(&a, st.handle())) refuse("cache_accept", rc);
+  written(kp);
+  written(vp);
+  if (v[6] != Py_None) written(out);
   return THPVariable_Wrap(out);
 }
 

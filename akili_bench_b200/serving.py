@@ -13,7 +13,9 @@ prompts and to decode over a paged key/value cache:
 Tensors are CUDA tensors on the current device, of any strides with a
 contiguous last axis; index tensors are int32 (slots int64).  Wrong types,
 shapes or devices raise TypeError or ValueError before the launch; the C
-entry's own refusals raise ``abi.AkiliError``.  Calls run on ``stream``
+entry's own refusals raise ``abi.AkiliError``.  The operators have no
+autograd formulas: results of inputs that require gradients raise in a backward
+pass (a cache's pages carry no history).  Calls run on ``stream``
 (default: the current stream) and do not synchronise; what they return is
 allocated on that stream, so a stream whose inputs are ready needs to wait for
 nothing else.

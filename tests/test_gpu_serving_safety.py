@@ -264,3 +264,85 @@ def test_scales_that_are_refused():
         with pytest.raises(abi.AkiliError) as e:
             ops.prompt_attention(q, q, q, i32([0, 4]), softmax_scale=scale)
         assert e.value.code == abi.E_UNSUPPORTED
+
+
+# ----------------------------------------------------------------- gradients --
+def tracked(*shape, dtype=F16):
+    """A tensor that is part of a graph, and the leaf it comes from."""
+    leaf = torch.randn(shape, device="cuda", dtype=dtype, requires_grad=True)
+    return leaf * 1, leaf
+
+
+def test_results_of_tracked_inputs_raise_in_a_backward_pass():
+    q, leaf = tracked(8, 2, 64)
+    plain = q.detach()
+    pos, table = torch.arange(8, dtype=torch.int32, device="cuda"), ops.rope_table(8, 64)
+    pages = torch.zeros(2, 16, 2, 64, device="cuda", dtype=F16)
+    v_pages, slots = pages.clone(), torch.arange(8, device="cuda")
+    tree = lambda x: ops.tree_attention(x, pages, v_pages, i32([[0, 1]]), i32([3]), i32([0, 8]),  # noqa: E731
+                                        return_lse=True)
+    calls = {
+        "inverse=True": lambda x: ops.rope(x, x, pos, table),
+        "rope_append": lambda x: (ops.rope_append(x, x, x, pos, table, slots, pages, v_pages),),
+        "prompt_attention": lambda x: ops.prompt_attention(x, x, x, i32([0, 8]), return_lse=True),
+        "tree_attention": tree,
+    }
+    for name, call in calls.items():
+        want = call(plain)
+        got = call(q)
+        for y, w in zip(got, want):
+            assert y.requires_grad and not w.requires_grad and torch.equal(y, w)
+            with pytest.raises(RuntimeError, match=name):
+                y.sum().backward(retain_graph=True)
+        with torch.no_grad():
+            assert not any(y.requires_grad for y in call(q))
+    assert leaf.grad is None and not pages.requires_grad and not v_pages.requires_grad
+    # the output of a call may be part of the graph as well
+    out = torch.empty_like(plain)
+    assert ops.prompt_attention(plain, q, plain, i32([0, 8]), out=out) is out and out.requires_grad
+    with pytest.raises(RuntimeError, match="prompt_attention"):
+        out.sum().backward()
+
+
+def test_values_that_were_saved_for_a_backward_pass_are_not_overwritten_unnoticed():
+    pos, table = torch.arange(8, dtype=torch.int32, device="cuda"), ops.rope_table(8, 64)
+    x, _ = tracked(8, 2, 64)
+    y = (x * x).sum()
+    ops.rope(x, x[:, :0], pos, table, q_out=x)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+    leaf = torch.randn(8, 2, 64, device="cuda", dtype=F16, requires_grad=True)
+    before = leaf.detach().clone()
+    with pytest.raises(RuntimeError, match="leaf"):
+        ops.rope(leaf, leaf[:, :0], pos, table, q_out=leaf)
+    assert torch.equal(leaf, before)
+    with torch.no_grad():
+        ops.rope(leaf, leaf[:, :0], pos, table, q_out=leaf)
+
+
+def test_tensors_written_in_place_get_a_new_version():
+    new = lambda *s: torch.zeros(s, device="cuda", dtype=F16)  # noqa: E731
+    q, k, v, pages, v_pages, out = new(8, 2, 64), new(8, 2, 64), new(8, 2, 64), new(2, 16, 2, 64), new(2, 16, 2, 64), \
+        new(8, 2, 64)
+    pos, table, slots = torch.arange(8, dtype=torch.int32, device="cuda"), ops.rope_table(8, 64), \
+        torch.arange(8, device="cuda")
+    lens = i32([0])
+    calls = [
+        (lambda: ops.rope(q, k, pos, table, q_out=q, k_out=k), (q, k)),
+        (lambda: ops.rope_append(q, k, v, pos, table, slots, pages, v_pages, q_out=out, k_out=k), (out, k, pages, v_pages)),
+        (lambda: ops.prompt_attention(q, k, v, i32([0, 8]), out=out), (out,)),
+        (lambda: ops.tree_attention(q, pages, v_pages, i32([[0, 1]]), i32([3]), i32([0, 8]), out=out), (out,)),
+        (lambda: ops.cache_accept(pages, v_pages, i32([[0, 1]]), i32([3]), i32([[1]]), i32([1]), new_lens=lens),
+         (pages, v_pages, lens)),
+    ]
+    every = (q, k, v, pages, v_pages, out, lens)
+    for call, changed in calls:
+        before = [t._version for t in every]
+        call()
+        for t, old in zip(every, before):
+            assert (t._version > old) == any(t is c for c in changed)
+    with torch.inference_mode():
+        x = torch.zeros(8, 2, 64, device="cuda", dtype=F16)
+        ops.rope(x, x[:, :0], pos, table, q_out=x)
+        ops.rope(q, k, pos, table, q_out=q, k_out=k)
+    ops.rope(x, x[:, :0], pos, table, q_out=x)  # (an inference tensor has no version)
