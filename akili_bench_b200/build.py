@@ -48,6 +48,16 @@ def _sources():
         [os.path.join(ROOT, "include", h) for h in ("akili.h", "akili_serving.h")]
 
 
+def _torch_dir() -> str:
+    return os.path.dirname(importlib.util.find_spec("torch").origin)
+
+
+def _serving_sources():
+    """The module is made of its source and headers, and of the torch that it was compiled against."""
+    return [os.path.join(CSRC, "serving_torch.cpp"), os.path.join(_torch_dir(), "version.py")] + \
+        [os.path.join(ROOT, "include", h) for h in ("akili.h", "akili_serving.h")]
+
+
 def _stale(out: str, deps: list[str]) -> bool:
     if not os.path.exists(out):
         return True
@@ -80,9 +90,8 @@ def build(force: bool = False, verbose: bool = False) -> list[str]:
             if verbose:
                 print(" ".join(cmd))
             _run(cmd)
-    src = os.path.join(CSRC, "serving_torch.cpp")
-    if force or _stale(SERVING_MODULE, [src, os.path.join(ROOT, "include", "akili_serving.h")]):
-        torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    if force or _stale(SERVING_MODULE, _serving_sources()):
+        src, torch_dir = os.path.join(CSRC, "serving_torch.cpp"), _torch_dir()
         cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-I", os.path.join(ROOT, "include"), "-I",
                os.path.join(torch_dir, "include"), "-I", os.path.join(torch_dir, "include/torch/csrc/api/include"), "-I",
                sysconfig.get_paths()["include"], "-I", cuda_inc, src, "-o", SERVING_MODULE, "-L", HERE, "-lakili", "-L",

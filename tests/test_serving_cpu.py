@@ -187,3 +187,25 @@ def test_front_end_refuses_cpu_tensors_and_wrong_types():
         ops.prompt_attention(q, q, q, torch.tensor([0, 4], dtype=torch.int32))
     with pytest.raises(ValueError):
         ops.rope_table(10, 64, scaling="cubic")
+
+
+def test_the_front_end_is_rebuilt_when_what_it_is_made_of_changes(tmp_path):
+    """Its source, every header that it includes from here, and torch itself."""
+    torch = pytest.importorskip("torch")
+    from akili_bench_b200 import build
+    names = {os.path.realpath(p) for p in build._serving_sources()}
+    seen, todo = set(), [os.path.join(build.CSRC, "serving_torch.cpp")]
+    while todo:
+        path = os.path.realpath(todo.pop())
+        if path in seen:
+            continue
+        seen.add(path)
+        for h in re.findall(r'^#include "([^"]+)"', open(path).read(), flags=re.M):
+            todo.append(os.path.join(os.path.dirname(path), h))
+    assert seen <= names
+    assert os.path.realpath(os.path.join(os.path.dirname(torch.__file__), "version.py")) in names
+    out = tmp_path / "module.so"
+    out.touch()
+    for name in names:
+        os.utime(out, (os.path.getmtime(name) - 1,) * 2)
+        assert build._stale(str(out), [name])
