@@ -29,6 +29,15 @@ bool all_multiples(const int64_t (&st)[n], int64_t of) {
   return true;
 }
 
+// Whether an output's entries can lie apart: those of an axis with stride 0
+// would be written one over the other, in any order.
+template <size_t n>
+bool apart(const int64_t (&stride)[n], const uint64_t (&extent)[n]) {
+  for (size_t i = 0; i < n; ++i)
+    if (extent[i] > 1 && stride[i] == 0) return false;
+  return true;
+}
+
 // The serving kernels are programmatic dependents of whatever runs before
 // them: a decode step is a chain of them, each a few microseconds long, and
 // one may be dispatched and set up while the one before drains.  Each waits
@@ -90,6 +99,11 @@ int run_rope(const akili_rope_arg_t* a, bool append, cudaStream_t st) {
   if (a->k_heads && append && (rc = check_aligned({a->v_addr, a->k_pages_addr, a->v_pages_addr}, es))) return rc;
   if (append && a->k_out_addr % es) return AKILI_E_ALIGN;
   if (append && (rc = check_aligned({a->slots_addr}, 8))) return rc;
+  if (a->q_heads && !apart(a->q_out_stride, {a->tokens, a->q_heads})) return AKILI_E_SHAPE;
+  if (a->k_heads && (!append || a->k_out_addr) && !apart(a->k_out_stride, {a->tokens, a->k_heads})) return AKILI_E_SHAPE;
+  if (a->k_heads && append && (!apart(a->k_page_stride, {a->num_pages, a->page_size, a->k_heads}) ||
+                               !apart(a->v_page_stride, {a->num_pages, a->page_size, a->k_heads})))
+    return AKILI_E_SHAPE;
   DevInfo di;
   if ((rc = device_info(&di))) return rc;
   RopeArgs r{};
@@ -245,6 +259,9 @@ int run_cache_accept(const akili_cache_accept_arg_t* a, cudaStream_t st) {
   if ((rc = check_aligned({a->page_table_addr, a->context_lens_addr, a->n_accepted_addr}, 4))) return rc;
   if (a->max_accepted && (rc = check_aligned({a->accepted_addr}, 4))) return rc;
   if (a->new_lens_addr % 4) return AKILI_E_ALIGN;
+  if (!apart(a->k_page_stride, {a->layers, a->num_pages, a->page_size, a->kv_heads}) ||
+      !apart(a->v_page_stride, {a->layers, a->num_pages, a->page_size, a->kv_heads}))
+    return AKILI_E_SHAPE;
   // one block writes a sequence's new length while others still read what the moves go by
   const uint64_t out = a->new_lens_addr, n = a->batch;
   if (ints_overlap(a->context_lens_addr, 1, n, 0, out, n) || ints_overlap(a->n_accepted_addr, 1, n, 0, out, n) ||
@@ -436,7 +453,7 @@ int run_prompt_attention(const akili_prompt_attention_arg_t* a, cudaStream_t st)
       !all_multiples(a->o_stride, 8))
     return AKILI_E_ALIGN;
   if (!loadable(a->q_stride, {a->total_q, a->q_heads}) || !loadable(a->k_stride, {a->total_k, a->kv_heads}) ||
-      !loadable(a->v_stride, {a->total_k, a->kv_heads}))
+      !loadable(a->v_stride, {a->total_k, a->kv_heads}) || !loadable(a->o_stride, {a->total_q, a->q_heads}))
     return AKILI_E_SHAPE;
   DevInfo di;
   if ((rc = device_info(&di))) return rc;
@@ -520,7 +537,8 @@ int run_tree_attention(const akili_tree_attention_arg_t* a, cudaStream_t st) {
     return AKILI_E_ALIGN;
   if (!loadable(a->q_stride, {a->total_q, a->q_heads}) ||
       !loadable(a->k_page_stride, {a->num_pages, a->page_size, a->kv_heads}) ||
-      !loadable(a->v_page_stride, {a->num_pages, a->page_size, a->kv_heads}))
+      !loadable(a->v_page_stride, {a->num_pages, a->page_size, a->kv_heads}) ||
+      !loadable(a->o_stride, {a->total_q, a->q_heads}))
     return AKILI_E_SHAPE;
   DevInfo di;
   if ((rc = device_info(&di))) return rc;

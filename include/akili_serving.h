@@ -19,7 +19,8 @@
  * Calls are asynchronous on `stream` and return AKILI_OK or an AKILI_E_*
  * code, like those of akili.h; arguments are checked before any CUDA call.
  * The caller owns every buffer.  Strides are in elements; the innermost
- * (head_dim) axis is contiguous.  Lengths, indices and masks live on the
+ * (head_dim) axis is contiguous; what is written has no stride of 0 along an
+ * axis of more than one entry.  Lengths, indices and masks live on the
  * device and are not read by the host: one that is out of range makes no
  * access outside the buffers: lengths are clamped to what the buffers hold,
  * entries are skipped, and where an entry's comment says so

@@ -170,6 +170,38 @@ def test_cache_accept_refuses_new_lengths_over_what_it_reads(read, cols, stride)
             assert code("cache_accept", a) == abi.E_NO_DEVICE, (read, at)
 
 
+def accept_arg(**kw):
+    a = abi.CacheAcceptArg(2, 4, 3, 2, 64, 50, 16, 7, 8, 0, A, A, A, A, A, A, 2 * A, 102400, 2048, 128, 64, 102400, 2048,
+                           128, 64, 7, 8)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("op,make,extents", [
+    ("rope", rope_arg, {"q_out_stride_token": "tokens", "q_out_stride_head": "q_heads", "k_out_stride_token": "tokens",
+                        "k_out_stride_head": "k_heads"}),
+    ("rope_append", rope_arg, {"q_out_stride_head": "q_heads", "k_out_stride_token": "tokens",
+                               "k_page_stride_page": "num_pages", "k_page_stride_token": "page_size",
+                               "v_page_stride_token": "page_size", "v_page_stride_head": "k_heads"}),
+    ("prompt_attention", prompt_arg, {"o_stride_token": "total_q", "o_stride_head": "q_heads"}),
+    ("tree_attention", tree_arg, {"o_stride_token": "total_q", "o_stride_head": "q_heads"}),
+    ("cache_accept", accept_arg, {"k_page_stride_layer": "layers", "k_page_stride_page": "num_pages",
+                                  "v_page_stride_token": "page_size", "v_page_stride_head": "kv_heads"})])
+def test_outputs_whose_entries_lie_over_one_another_are_refused(op, make, extents):
+    """Stride 0 along a written axis; along an axis of one entry it is never used."""
+    torch = pytest.importorskip("torch")
+    for stride, extent in extents.items():
+        assert code(op, make(**{stride: 0})) == abi.E_SHAPE, stride
+        if not torch.cuda.is_available():
+            one = {extent: 1}
+            if extent == "q_heads" and op.endswith("attention"):
+                one["kv_heads"] = 1
+            if extent == "page_size" and op == "cache_accept":
+                one["max_pages"] = 1
+            assert code(op, make(**{stride: 0}, **one)) == abi.E_NO_DEVICE, stride
+
+
 def test_valid_blocks_without_a_gpu_report_no_device():
     torch = pytest.importorskip("torch")
     if torch.cuda.is_available():
