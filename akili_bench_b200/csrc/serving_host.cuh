@@ -63,15 +63,19 @@ int launch_dependent(void (*kern)(Params...), dim3 grid, int threads, int smem, 
 }
 
 // ------------------------------------------------------------------- rope --
+// Blocks that share a token's heads, at most `most`: with few tokens as many as fill the GPU.
+constexpr int rope_shares(int tokens, int most, int sms) {
+  const int64_t want = (4ll * sms + tokens - 1) / tokens;
+  return static_cast<int>(std::min<int64_t>({most, want, 65535}));
+}
+static_assert(rope_shares(1, 9, 148) == 9 && rope_shares(100, 9, 148) == 6 && rope_shares(INT32_MAX, 9, 148) == 1);
+
 template <typename T, int VEC, bool kAppend>
 int launch_rope(const DevInfo& di, const RopeArgs& r, cudaStream_t st) {
   const int units = r.rot_dim / 2 / VEC + (r.head_dim - r.rot_dim + 2 * VEC - 1) / (2 * VEC);
   const int hl = kRopeThreads / std::min(units, kRopeThreads);
   const int heads = r.q_heads + r.k_heads * (kAppend ? 2 : 1);
-  // few tokens: the heads of one are shared among as many blocks as they fill
-  const int most = (heads + hl - 1) / hl;
-  const int want = (4 * di.sms + r.tokens - 1) / r.tokens;
-  const dim3 grid(r.tokens, std::min({most, want, 65535}));
+  const dim3 grid(r.tokens, rope_shares(r.tokens, (heads + hl - 1) / hl, di.sms));
   return launch_dependent(rope_kernel<T, VEC, kAppend>, grid, kRopeThreads, 0, st, r);
 }
 
