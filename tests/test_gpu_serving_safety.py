@@ -1,6 +1,10 @@
 """The serving operators where calls meet: waits that give up, streams, captured
 graphs, buffers that overlap, requests a default could hide."""
 import ctypes as C
+import os
+import subprocess
+import sys
+import threading
 
 import pytest
 
@@ -346,3 +350,94 @@ def test_tensors_written_in_place_get_a_new_version():
         ops.rope(x, x[:, :0], pos, table, q_out=x)
         ops.rope(q, k, pos, table, q_out=q, k_out=k)
     ops.rope(x, x[:, :0], pos, table, q_out=x)  # (an inference tensor has no version)
+
+
+# ------------------------------------------------------------ batches, order --
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("new,context", [([1] * 9 + [200] + [1] * 6, 300),      # the 64-row form: the chunk in many items
+                                         ([1, 500, 1, 1], 130),                 # the 256-row form: single tokens too
+                                         ([1, 1, 60, 1, 1, 1, 1, 1], 700)])     # 64 rows, cut items
+def test_a_chunk_among_single_tokens(dtype, new, context):
+    g = torch.Generator().manual_seed(sum(new))
+    heads, hk, d, page = 8, 2, 128, 16
+    lens = [(context * (b + 3) * 7) % (2 * context) for b in range(len(new))]
+    per = -(-max(c + n for c, n in zip(lens, new)) // page)
+    table = torch.randperm(len(new) * per, generator=g).to(torch.int32).view(len(new), per)
+    kp, vp = (torch.randn(len(new) * per, page, hk, d, generator=g).to(dtype) for _ in range(2))
+    q = torch.randn(sum(new), heads, d, generator=g).to(dtype)
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    got, lse = ops.tree_attention(q.cuda(), kp.cuda(), vp.cuda(), table.cuda(), i32(lens), i32(cu), return_lse=True)
+    for b, (c, n) in enumerate(zip(lens, new)):
+        k, v = (p[table[b].long()].flatten(0, 1)[:c + n] for p in (kp, vp))
+        o, l, bound, l_bound = ref.attend(q[cu[b]:cu[b + 1]], k, v, ref.causal(n, c + n))
+        ref.assert_within(got[cu[b]:cu[b + 1]], o, bound, f"sequence {b}")
+        ref.assert_within(lse[cu[b]:cu[b + 1]], l, l_bound, f"lse of sequence {b}")
+
+
+def test_two_threads_on_one_stream():
+    """The scratch of the stream is shared, the calls of the front end take turns."""
+    sizes = [step(1, 8, 900), step(60, 8, 700), step(9, 4, 400)]
+    want = [ops.tree_attention(*s) for s in sizes]
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(first):
+        with torch.cuda.stream(stream):
+            got = [(i % 3, ops.tree_attention(*sizes[i % 3])) for i in range(first, first + 60)]
+            stream.synchronize()
+            wrong.extend(i for i, o in got if not torch.equal(o, want[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+CHAIN = """
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+from akili_bench_b200 import ops
+g = torch.Generator("cuda").manual_seed(5)
+r = lambda *s: torch.randn(s, generator=g, device="cuda", dtype=torch.float16)
+i = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+pages, v_pages, table = r(40, 16, 2, 64), r(40, 16, 2, 64), ops.rope_table(512, 64)
+page_table = torch.arange(40, dtype=torch.int32, device="cuda").view(2, 20)
+lens, cu, out = i([0, 0]), i([0, 30, 70]), []
+pos = torch.cat([torch.arange(30), torch.arange(40)]).int().cuda()
+slots = torch.cat([torch.arange(30), torch.arange(40) + 320]).cuda()
+q, k, v = r(70, 8, 64), r(70, 2, 64), r(70, 2, 64)
+q = ops.rope_append(q, k, v, pos, table, slots, pages, v_pages, k_out=k)
+out.append(ops.prompt_attention(q, k, v, cu))
+lens = i([30, 40])
+for s in range(20):  # each call's inputs are the results of the one before
+    cu = i([0, 4, 8])
+    mask = ops.tree_mask(i([-1, 0, 0, 2] * 2), cu, 4)
+    base = torch.stack([lens, lens + 320], 1)
+    at = (base[:, 1:] + torch.arange(4, device="cuda") + torch.tensor([[0], [0]], device="cuda"))
+    at[0] -= 320
+    x = out[-1][:8]
+    q = ops.rope_append(x, x[:, :2], x[:, 2:4], i([0, 1, 1, 2] * 2), table, at.flatten().long(), pages, v_pages)
+    out.append(ops.tree_attention(q, pages, v_pages, page_table, lens, cu, mask))
+    lens = ops.cache_accept(pages, v_pages, page_table, lens, i([[0, 2, 3]] * 2), i([3, 2]))
+out += [lens, pages, v_pages]
+torch.save([t.cpu() for t in out], sys.argv[2])
+assert ops.device_status() == 0
+"""
+
+
+def test_dependent_launches_give_what_plain_ones_do(tmp_path):
+    """A chain of calls, each on the results of the one before, with AKILI_PDL=0 and 1: equal bits."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    got = []
+    for pdl in "01":
+        path = str(tmp_path / pdl)
+        subprocess.run([sys.executable, "-c", CHAIN, root, path], check=True, timeout=300,
+                       env=dict(os.environ, AKILI_PDL=pdl))
+        got.append(torch.load(path))
+    assert len(got[0]) == 24 and all(torch.equal(a, b) for a, b in zip(*got))
+    assert got[0][21].tolist() == [90, 80] and not any(torch.isnan(t.float()).any() for t in got[0])
