@@ -21,7 +21,9 @@ __device__ __forceinline__ int find_sequence(const int* cu, int batch, int t) {
 }
 
 // One thread per node walks up to its root.  A parent is smaller than its
-// child, so the walk ends; one that is not ends it and is recorded.
+// child, so the walk ends; one that is not ends it and is recorded.  Bound by
+// the dependent loads of the longest branch: 16 trees of 16 to 64 nodes 3.5 us,
+// 16 chains of 64 nodes 8.3 us.
 __global__ void __launch_bounds__(128) tree_mask_kernel(const int* parents, const int* cu_q, unsigned int* mask,
                                                         int batch, int total, int words) {
   griddep_wait();
@@ -69,7 +71,7 @@ constexpr int kAcceptRows = 128;  // moves whose offsets are held at a time
 // the entry whose destination it is, or in the same batch, whose loads all
 // come before its stores.  Bound by its chain of latencies (lengths, indices,
 // pages, values): 16 sequences, 87 entries, 32 layers of 8 heads of 128 take
-// 5.5 us, 22 MB.
+// 5.9 us, 22 MB.
 template <typename U>
 __global__ void __launch_bounds__(kAcceptThreads) cache_accept_kernel(const AcceptArgs a) {
   griddep_wait();

@@ -51,11 +51,14 @@
 //
 // Bound by the chain of a block: scores, TMEM load, maximum, exponentials, P,
 // product.  One stream alone would take 2300 cycles a block; the two overlap to
-// 60% of the tensor pipe (and of the exponential unit; without exponentials
-// the time is the same).  Measured: 8 causal prompts of 4096 tokens, 32 heads
-// of 128, fp16: 1.21 ms, 907 TFLOP/s of visible pairs; six uneven bf16 prompts
-// with 32/8 heads: 945 TFLOP/s; 24 short ones with 14/2 heads of 64: 12 us; 16
-// drafted trees over 700 to 5999 tokens: 73 us (79 with nothing in L2).
+// 60% of the tensor pipe (and of the exponential unit; a copy without
+// exponentials took the same time, at a clock that was not recorded).
+// Measured: 8 causal prompts of 4096 tokens, 32 heads of 128, fp16: 1.19 ms, 925
+// TFLOP/s of visible pairs; six uneven bf16 prompts with 32/8 heads: 949
+// TFLOP/s; 24 short ones with 14/2 heads of 64: 12 us; 16 drafted trees over 700
+// to 5999 tokens: 73 us (77 with nothing in L2).  Of the 96 registers that 640
+// threads leave, the single-tile forms spill 22 to 32 bytes a thread, the paged
+// pair form 12 to 16.
 #pragma once
 #include <type_traits>
 
@@ -217,7 +220,6 @@ __device__ __forceinline__ long long warp_scan(long long v) {  // inclusive
   return v;
 }
 
-// Blocks of sequence b on the line (0 past the batch).
 // Sequence b's place on the line (no blocks past the batch).
 template <int kTileRows>
 __device__ __forceinline__ void sv_line_sequence(const ServingArgs& a, int b, bool record, SvWalk<kTileRows>& w) {
@@ -1037,6 +1039,7 @@ __global__ void __maxnreg__(96)
             f2_unpack(f2_fma(f2_pack(s[2 * x], s[2 * x + 1]), sl2, nm2), x0, x1);
             const float p0 = ex2_mufu(x0), p1 = ex2_mufu(x1);
             sm2[x & 3] = f2_add(sm2[x & 3], f2_pack(p0, p1));
+            // (rounded to the element type: a 16-bit product takes 16-bit operands; the sums keep fp32)
             pk[y] = pack2<T>(p0, p1);
           }
           tmem_st_p(tP + p * kPPairs, pk);

@@ -104,7 +104,8 @@ int run_rope(const akili_rope_arg_t* a, bool append, cudaStream_t st) {
   if (append && a->k_out_addr % es) return AKILI_E_ALIGN;
   if (append && (rc = check_aligned({a->slots_addr}, 8))) return rc;
   if (a->q_heads && !apart(a->q_out_stride, {a->tokens, a->q_heads})) return AKILI_E_SHAPE;
-  if (a->k_heads && (!append || a->k_out_addr) && !apart(a->k_out_stride, {a->tokens, a->k_heads})) return AKILI_E_SHAPE;
+  if (a->k_heads && (!append || a->k_out_addr) && !apart(a->k_out_stride, {a->tokens, a->k_heads}))
+    return AKILI_E_SHAPE;
   if (a->k_heads && append && (!apart(a->k_page_stride, {a->num_pages, a->page_size, a->k_heads}) ||
                                !apart(a->v_page_stride, {a->num_pages, a->page_size, a->k_heads})))
     return AKILI_E_SHAPE;

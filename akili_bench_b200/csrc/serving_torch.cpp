@@ -3,7 +3,9 @@
 //
 // The operators of a decode step run for a few microseconds, so the front end
 // has to cost less than that: checking and filling the argument blocks from
-// Python took 15 to 25 us a call, here about 2.  akili_bench_b200/serving.py
+// Python took 15 to 25 us a call; here a call takes the host 3.5 to 5 us, the
+// launch included (tree_attention, with its tensor maps and two launches, 8.5).
+// akili_bench_b200/serving.py
 // holds the documented functions; each passes its arguments on by position.
 // Wrong types, shapes and devices raise TypeError or ValueError; a refusal of
 // the C entry raises abi.AkiliError.

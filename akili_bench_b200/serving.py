@@ -10,15 +10,19 @@ prompts and to decode over a paged key/value cache:
   chunks, drafted trees) over the cache;
 * ``cache_accept`` — compaction of the accepted branch after verification.
 
-Tensors are CUDA tensors on the current device, of any strides with a
-contiguous last axis; index tensors are int32 (slots int64).  Wrong types,
-shapes or devices raise TypeError or ValueError before the launch; the C
-entry's own refusals raise ``abi.AkiliError``.  The operators have no
-autograd formulas: results of inputs that require gradients raise in a backward
-pass (a cache's pages carry no history).  Calls run on ``stream``
-(default: the current stream) and do not synchronise; what they return is
-allocated on that stream, so a stream whose inputs are ready needs to wait for
-nothing else.
+Tensors are CUDA tensors on the current device with a contiguous last axis;
+index tensors are int32 (slots int64).  The other strides are free for the
+rotations and ``cache_accept`` (written axes may not be broadcast).  The
+attentions load tiles: their q, k, v, pages and outputs start on 16 bytes, with
+positive strides that are multiples of 8 elements.  Wrong types, shapes or
+devices raise TypeError or ValueError before the launch; the C entry's own
+refusals raise ``abi.AkiliError``.
+
+Calls run on ``stream`` (default: the current stream) and do not synchronise;
+what they return is allocated on that stream, so a stream whose inputs are ready
+needs to wait for nothing else.  The operators have no autograd formulas:
+results of inputs that require gradients raise in a backward pass (a cache's
+pages carry no history).
 """
 from __future__ import annotations
 
@@ -76,7 +80,9 @@ def rope(q, k, positions, table, interleaved: bool = False, inverse: bool = Fals
     k [tokens, k_heads, head_dim] by the angles of their positions (int32 [tokens]).
 
     Pairs are (i, i + rot_dim/2), or (2i, 2i + 1) when interleaved.  inverse=True rotates back: it is the
-    gradient (apply it to dq, dk).  q_out/k_out may be q/k (in place).  Returns (q_out, k_out)."""
+    gradient (apply it to dq, dk).  q_out/k_out may be q/k (in place).  A token whose position is outside the
+    table is skipped and recorded (``ops.device_status``): its output rows are not written, so that new ones hold
+    anything.  Returns (q_out, k_out)."""
     return _native.rope(q, k, positions, table, interleaved, inverse, q_out, k_out, stream)
 
 
@@ -85,7 +91,8 @@ def rope_append(q, k, v, positions, table, slots, k_pages, v_pages, interleaved:
     """`rope`, with the rotated k and v [tokens, k_heads, head_dim] written to row slots[token] = page *
     page_size + offset (int64; -1: padding, nothing is written) of k_pages/v_pages [num_pages, page_size,
     k_heads, head_dim].  k_out, if given, gets the rotated k as well (`prompt_attention` of the same prompt
-    reads it; it may be k).  Returns the rotated q (q_out; may be q)."""
+    reads it; it may be k).  A token whose position is outside the table is skipped and recorded: nothing is
+    written for it, and its rows of a new q_out hold anything.  Returns the rotated q (q_out; may be q)."""
     return _native.rope_append(q, k, v, positions, table, slots, k_pages, v_pages, interleaved, q_out, k_out, stream)
 
 
@@ -96,7 +103,9 @@ def prompt_attention(q, k, v, cu_q, cu_k=None, softmax_scale: float | None = Non
 
     With n queries and m keys, query i sees the keys j <= i + m - n (causal) or all; one that sees none gives
     0.  Query head h reads key head h // (q_heads // kv_heads).  softmax_scale defaults to head_dim**-0.5;
-    0.0 weighs all visible keys alike.  Returns out, or (out, lse) with lse fp32 [total_q, q_heads] (natural log, -inf for a row without keys)."""
+    0.0 weighs all visible keys alike.  Rows past the last sequence are not written (in a new out and lse they hold
+    anything).  Returns out, or (out, lse) with lse fp32 [total_q, q_heads] (natural log, -inf for a row without
+    keys)."""
     return _native.prompt_attention(q, k, v, cu_q, cu_k, softmax_scale, causal, out, return_lse, stream)
 
 
@@ -115,7 +124,8 @@ def tree_attention(q, k_pages, v_pages, page_table, context_lens, cu_q, mask=Non
     and values already follow its context_lens[b] sure tokens in the cache (`rope_append`).  Entry j lies in
     row j % page_size of page page_table[b, j // page_size] of k_pages/v_pages [num_pages, page_size, kv_heads,
     head_dim] (any strides, page_size a multiple of 8).  Every new token sees the context and the new tokens
-    of its mask row (`tree_mask`); without a mask, itself and those before it (a single token, a chunk).
+    of its mask row (`tree_mask`); without a mask, itself and those before it (a single token, a chunk).  Rows past
+    the last sequence are not written (in a new out and lse they hold anything).
     Returns out, or (out, lse); `workspace` is an optional uint8 tensor of tree_attention_workspace() bytes."""
     return _native.tree_attention(q, k_pages, v_pages, page_table, context_lens, cu_q, mask, softmax_scale, out,
                                   return_lse, workspace, stream)

@@ -158,8 +158,8 @@ def step(tokens, group, context, dtype=F16, pages=64):
 def c_entry(args, out, stream, workspace=None):
     """akili_tree_attention itself, without the torch front end."""
     q, kp, vp, table, lens, cu = args
-    a = abi.TreeAttentionArg(abi.DTYPE_F16, q.shape[1], 1, 128, 2, q.shape[0], kp.shape[0], 16, table.shape[1], 0, 0.0, 0,
-                             q.data_ptr(), kp.data_ptr(), vp.data_ptr(), out.data_ptr(), 0, table.data_ptr(),
+    a = abi.TreeAttentionArg(abi.DTYPE_F16, q.shape[1], 1, 128, 2, q.shape[0], kp.shape[0], 16, table.shape[1], 0, 0.0,
+                             0, q.data_ptr(), kp.data_ptr(), vp.data_ptr(), out.data_ptr(), 0, table.data_ptr(),
                              lens.data_ptr(), cu.data_ptr(), 0, 0, 0, *q.stride()[:2], *out.stride()[:2],
                              *kp.stride()[:3], *vp.stride()[:3], table.stride(0), 0)
     if workspace is not None:
@@ -333,7 +333,8 @@ def test_tensors_written_in_place_get_a_new_version():
     lens = i32([0])
     calls = [
         (lambda: ops.rope(q, k, pos, table, q_out=q, k_out=k), (q, k)),
-        (lambda: ops.rope_append(q, k, v, pos, table, slots, pages, v_pages, q_out=out, k_out=k), (out, k, pages, v_pages)),
+        (lambda: ops.rope_append(q, k, v, pos, table, slots, pages, v_pages, q_out=out, k_out=k),
+         (out, k, pages, v_pages)),
         (lambda: ops.prompt_attention(q, k, v, i32([0, 8]), out=out), (out,)),
         (lambda: ops.tree_attention(q, pages, v_pages, i32([[0, 1]]), i32([3]), i32([0, 8]), out=out), (out,)),
         (lambda: ops.cache_accept(pages, v_pages, i32([[0, 1]]), i32([3]), i32([[1]]), i32([1]), new_lens=lens),
@@ -354,9 +355,9 @@ def test_tensors_written_in_place_get_a_new_version():
 
 # ------------------------------------------------------------ batches, order --
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("new,context", [([1] * 9 + [200] + [1] * 6, 300),      # the 64-row form: the chunk in many items
-                                         ([1, 500, 1, 1], 130),                 # the 256-row form: single tokens too
-                                         ([1, 1, 60, 1, 1, 1, 1, 1], 700)])     # 64 rows, cut items
+@pytest.mark.parametrize("new,context", [([1] * 9 + [200] + [1] * 6, 300),   # 64 rows: the chunk in many items
+                                         ([1, 500, 1, 1], 130),              # 256 rows: single tokens too
+                                         ([1, 1, 60, 1, 1, 1, 1, 1], 700)])  # 64 rows, cut items
 def test_a_chunk_among_single_tokens(dtype, new, context):
     g = torch.Generator().manual_seed(sum(new))
     heads, hk, d, page = 8, 2, 128, 16
